@@ -1,0 +1,122 @@
+"""Loader for libfedtrain.so, the dense training operators' C-ABI
+(include/fedtrain.h).  As with libfedagg (``_native``), torch's HIP runtime is
+mapped first and there is no fallback: a missing library raises.
+"""
+from __future__ import annotations
+
+import ctypes
+import os
+import threading
+
+import torch  # noqa: F401  (must precede the dlopen below)
+
+from ._native import FedAggError, _hip_runtimes_mapped
+
+_HERE = os.path.dirname(os.path.abspath(__file__))
+LIB_PATH = os.environ.get("FEDTRAIN_LIB", os.path.join(_HERE, "libfedtrain.so"))
+
+# Must match include/fedtrain.h
+ABI_VERSION = 1
+FEDTRAIN_EINVAL = -22
+FEDTRAIN_F32, FEDTRAIN_BF16, FEDTRAIN_F16 = 0, 1, 2
+FEDTRAIN_ACT_NONE, FEDTRAIN_ACT_RELU, FEDTRAIN_ACT_GELU, FEDTRAIN_ACT_SILU = 0, 1, 2, 3
+FEDTRAIN_FORWARD, FEDTRAIN_GRAD_INPUT, FEDTRAIN_GRAD_WEIGHT = 0, 1, 2
+
+
+class ProductArgs(ctypes.Structure):
+    """struct fedtrain_product_args (include/fedtrain.h)."""
+
+    _fields_ = ([(n, ctypes.c_int32) for n in ("dtype", "form", "act", "groups")]
+                + [(n, ctypes.c_int64) for n in ("m", "n", "k")]
+                + [("a", ctypes.c_void_p), ("lda", ctypes.c_int64),
+                   ("b", ctypes.c_void_p), ("ldb", ctypes.c_int64), ("b_group", ctypes.c_int64),
+                   ("c", ctypes.c_void_p), ("ldc", ctypes.c_int64), ("c_group", ctypes.c_int64),
+                   ("bias", ctypes.c_void_p), ("bias_group", ctypes.c_int64),
+                   ("res", ctypes.c_void_p), ("ldr", ctypes.c_int64),
+                   ("z", ctypes.c_void_p), ("ldz", ctypes.c_int64),
+                   ("colsum", ctypes.c_void_p), ("colsum_group", ctypes.c_int64),
+                   ("offsets", ctypes.c_void_p), ("offsets64", ctypes.c_int32),
+                   ("reserved", ctypes.c_int32),
+                   ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64)])
+
+
+class AdamWScalars(ctypes.Structure):
+    """struct fedtrain_adamw_scalars (include/fedtrain.h)."""
+
+    _fields_ = ([(n, ctypes.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay")]
+                + [("step", ctypes.c_int64), ("seed", ctypes.c_uint32),
+                   ("maximize", ctypes.c_int32), ("device_step", ctypes.c_void_p),
+                   ("workspace", ctypes.c_void_p)])
+
+
+# struct fedtrain_adamw_tensor as eight 64-bit words: p, g, m, v, m_scale,
+# v_scale, n, block0
+ADAMW_WORDS = 8
+
+SIGNATURES = {
+    "fedtrain_abi_version": (ctypes.c_int, []),
+    "fedtrain_strerror": (ctypes.c_char_p, [ctypes.c_int]),
+    "fedtrain_product_workspace": (ctypes.c_int64, [ctypes.POINTER(ProductArgs)]),
+    "fedtrain_product": (ctypes.c_int, [ctypes.POINTER(ProductArgs), ctypes.c_void_p]),
+    "fedtrain_act_backward": (
+        ctypes.c_int,
+        [ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
+         ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,
+         ctypes.c_void_p],
+    ),
+    "fedtrain_adamw": (
+        ctypes.c_int,
+        [ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.c_void_p,
+         ctypes.POINTER(AdamWScalars), ctypes.c_void_p],
+    ),
+}
+
+_lock = threading.Lock()
+_lib = None
+
+
+def load():
+    """Load (once) and return the ctypes handle; raise if unavailable."""
+    global _lib
+    if _lib is not None:
+        return _lib
+    with _lock:
+        if _lib is not None:
+            return _lib
+        if not os.path.exists(LIB_PATH):
+            raise FedAggError(
+                f"{LIB_PATH} not found: build it with `python -c "
+                f"'import __graft_entry__ as g; g.build()'` (no CPU fallback exists)"
+            )
+        lib = ctypes.CDLL(LIB_PATH)
+        lib.fedtrain_abi_version.restype = ctypes.c_int
+        lib.fedtrain_abi_version.argtypes = []
+        built = lib.fedtrain_abi_version()
+        if built != ABI_VERSION:
+            raise FedAggError(f"{LIB_PATH} has ABI version {built}, this package needs "
+                              f"{ABI_VERSION}; rebuild the library")
+        for name, (res, args) in SIGNATURES.items():
+            try:
+                fn = getattr(lib, name)
+            except AttributeError:
+                raise FedAggError(f"{LIB_PATH} does not export {name}; rebuild the library") \
+                    from None
+            fn.restype = res
+            fn.argtypes = args
+        runtimes = _hip_runtimes_mapped()
+        if len(runtimes) > 1:
+            raise FedAggError("two HIP runtimes are mapped (%s); import torch before fedsim_amd"
+                              % sorted(runtimes))
+        _lib = lib
+        return lib
+
+
+def check(rc: int, what: str) -> None:
+    if rc != 0:
+        msg = load().fedtrain_strerror(rc).decode()
+        raise FedAggError(f"{what} failed ({rc}): {msg}")
+
+
+def exported_symbols():
+    """Names of the C-ABI entry points (the ones include/fedtrain.h declares)."""
+    return list(SIGNATURES)

@@ -1,0 +1,145 @@
+"""Optimizers whose step is one kernel (train_ops.adamw_step)."""
+from __future__ import annotations
+
+from typing import Iterable, Tuple
+
+import torch
+
+from . import train_ops
+
+__all__ = ["AdamW"]
+
+_STATES = {32: (torch.float32, torch.float32), 8: (torch.float8_e4m3fn, torch.float8_e5m2)}
+_NAMES = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")
+
+
+class AdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW's step (decoupled weight decay, bias correction) over
+    all parameters at once, on a HIP device.  An ``optimizer_def`` of it serves
+    the clients' local training and the server step alike.
+
+    ``state_bits=8`` holds the moments in e4m3 and e5m2 codes with a power of
+    two for each 256 elements: 2 bytes an element instead of 8.  The codes are
+    rounded stochastically from ``seed``, the step's number and the element's.
+
+    ``capturable=True`` counts the steps on the device, together for the
+    parameters of a group, so that a captured graph of ``step()`` goes on
+    counting when it is replayed; capture after the first eager step, which
+    makes the states.  Otherwise each parameter counts its own steps on the host
+    and a capture raises.
+
+    Parameters are contiguous float32, bfloat16 or float16 tensors; a 16-bit
+    parameter is rounded to nearest each step.  The step of a captured graph
+    uses the learning rate it was captured with."""
+
+    def __init__(self, params: Iterable, lr: float = 1e-3,
+                 betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, *, state_bits: int = 32, seed: int = 0,
+                 maximize: bool = False, capturable: bool = False):
+        if state_bits not in _STATES:
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        if not (lr >= 0 and 0 <= betas[0] < 1 and 0 <= betas[1] < 1 and eps >= 0
+                and weight_decay >= 0):
+            raise ValueError(f"lr {lr}, betas {betas}, eps {eps}, weight_decay {weight_decay}: "
+                             "betas lie in [0, 1), the others are not negative")
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps,
+                                      weight_decay=weight_decay, state_bits=state_bits, seed=seed,
+                                      maximize=maximize, capturable=capturable))
+
+    def _init_state(self, p, group, st):
+        m, v = _STATES[group["state_bits"]]
+        st["exp_avg"] = torch.zeros(p.shape, dtype=m, device=p.device)
+        st["exp_avg_sq"] = torch.zeros(p.shape, dtype=v, device=p.device)
+        if group["state_bits"] == 8:
+            blocks = -(-p.numel() // train_ops.STATE_BLOCK)
+            st["exp_avg_scale"] = torch.ones(blocks, dtype=torch.float32, device=p.device)
+            st["exp_avg_sq_scale"] = torch.ones(blocks, dtype=torch.float32, device=p.device)
+        st["step"] = 0
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        block = 0
+        for group in self.param_groups:
+            todo = {}  # (type, device, step) -> parameters of one call
+            for p in group["params"]:
+                first, block = block, block - (-p.numel() // train_ops.STATE_BLOCK)
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise RuntimeError("AdamW does not take sparse gradients")
+                train_ops._require(p, "a parameter")
+                if not p.is_contiguous():
+                    raise ValueError("a parameter must be contiguous")
+                st = self.state[p]
+                capturing = torch.cuda.is_current_stream_capturing()
+                if not st:
+                    if capturing:
+                        raise RuntimeError("take a step before capturing one: the first makes "
+                                           "the states")
+                    self._init_state(p, group, st)
+                if group["capturable"]:
+                    key = (p.dtype, p.device, None)
+                elif capturing:
+                    raise RuntimeError("AdamW counts its steps on the host: a captured graph "
+                                       "needs capturable=True")
+                else:
+                    st["step"] = int(st["step"]) + 1
+                    key = (p.dtype, p.device, st["step"])
+                todo.setdefault(key, []).append((p, st, first))
+            counted = {}
+            for (_, dev, n), items in todo.items():
+                if n is None:
+                    n = counted.get(dev)
+                    if n is None:
+                        n = counted[dev] = self._count(group, dev)
+                    for _, st, _ in items:
+                        st["step"] = n
+                eight = group["state_bits"] == 8
+                train_ops.adamw_step(
+                    [p for p, _, _ in items], [p.grad.contiguous() for p, _, _ in items],
+                    [st["exp_avg"] for _, st, _ in items],
+                    [st["exp_avg_sq"] for _, st, _ in items],
+                    [st["exp_avg_scale"] for _, st, _ in items] if eight else None,
+                    [st["exp_avg_sq_scale"] for _, st, _ in items] if eight else None,
+                    step=n, lr=float(group["lr"]), betas=group["betas"], eps=group["eps"],
+                    weight_decay=group["weight_decay"], maximize=group["maximize"],
+                    seed=group["seed"], first_blocks=[f for _, _, f in items])
+        return loss
+
+    def _count(self, group, dev) -> torch.Tensor:
+        """The group's step on ``dev``, one further: the tensor that every
+        parameter's state holds."""
+        n = None
+        for p in group["params"]:
+            st = self.state.get(p)
+            if st and p.device == dev and isinstance(st["step"], torch.Tensor):
+                n = st["step"]
+                break
+        if n is None:
+            known = [int(self.state[p]["step"]) for p in group["params"] if self.state.get(p)
+                     and p.device == dev]
+            n = torch.full((1,), max(known, default=0), dtype=torch.int64, device=dev)
+        n.add_(1)
+        return n
+
+    def load_state_dict(self, state_dict):
+        """torch's, with the states in their own types: torch would cast them
+        to the parameters'.  As there, the groups' options are the saved ones,
+        ``state_bits`` among them."""
+        super().load_state_dict(state_dict)
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        ps = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(ids, ps):
+            given = state_dict["state"].get(i)
+            if not given:
+                continue
+            st = self.state[p]
+            for name in _NAMES:
+                if name in given:
+                    st[name] = given[name].detach().to(p.device, copy=True)
+            if isinstance(given["step"], torch.Tensor):
+                st["step"] = int(given["step"])
