@@ -1,10 +1,12 @@
 """Loader for libfedtrain.so, the dense training operators' C-ABI
-(include/fedtrain.h).  As with libfedagg (``_native``), torch's HIP runtime is
-mapped first and there is no fallback: a missing library raises.
+(include/fedtrain.h), and for ``_fedtrain``, the module that calls it on torch
+tensors (csrc/fedtrain_binding.cpp).  As with libfedagg (``_native``), torch's
+HIP runtime is mapped first and there is no fallback: a missing library raises.
 """
 from __future__ import annotations
 
 import ctypes
+import importlib
 import os
 import threading
 
@@ -13,7 +15,7 @@ import torch  # noqa: F401  (must precede the dlopen below)
 from ._native import FedAggError, _hip_runtimes_mapped
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
-LIB_PATH = os.environ.get("FEDTRAIN_LIB", os.path.join(_HERE, "libfedtrain.so"))
+LIB_PATH = os.path.join(_HERE, "libfedtrain.so")
 
 # Must match include/fedtrain.h
 ABI_VERSION = 1
@@ -73,6 +75,20 @@ SIGNATURES = {
 
 _lock = threading.Lock()
 _lib = None
+_ext = None
+
+
+def ext():
+    """The module ``_fedtrain`` (loaded once); raise if unavailable."""
+    global _ext
+    if _ext is None:
+        load()
+        try:
+            _ext = importlib.import_module("._fedtrain", __package__)
+        except ImportError as e:
+            raise FedAggError(f"fedsim_amd._fedtrain cannot be loaded ({e}): build it with "
+                              "`python -c 'import __graft_entry__ as g; g.build()'`") from e
+    return _ext
 
 
 def load():
@@ -109,12 +125,6 @@ def load():
                               % sorted(runtimes))
         _lib = lib
         return lib
-
-
-def check(rc: int, what: str) -> None:
-    if rc != 0:
-        msg = load().fedtrain_strerror(rc).decode()
-        raise FedAggError(f"{what} failed ({rc}): {msg}")
 
 
 def exported_symbols():

@@ -71,9 +71,9 @@ class AdamW(torch.optim.Optimizer):
                     continue
                 if p.grad.is_sparse:
                     raise RuntimeError("AdamW does not take sparse gradients")
-                train_ops._require(p, "a parameter")
-                if not p.is_contiguous():
-                    raise ValueError("a parameter must be contiguous")
+                if p.device.type != "cuda" or not p.is_contiguous():
+                    raise ValueError("a parameter must be a contiguous tensor on a HIP device, "
+                                     f"got strides {p.stride()} on {p.device}")
                 st = self.state[p]
                 capturing = torch.cuda.is_current_stream_capturing()
                 if not st:

@@ -440,3 +440,35 @@ def test_only_what_is_asked_for():
                 assert torch.equal(g.cpu(), dy)
             else:
                 R.close(g, want[n], n)
+
+
+def test_a_second_derivative_is_refused():
+    from fedsim_amd.functional import linear_act
+
+    x, w, b, _, dy = _case(20, 24, 16, torch.float32, 21, residual=False)
+    X, W, B = (t.to(DEV).requires_grad_(True) for t in (x, w, b))
+    y = linear_act(X, W, B, activation="gelu")
+    dx, dw, db = torch.autograd.grad(y, (X, W, B), dy.to(DEV), create_graph=True)
+    want = R.product(_up(x), _up(w), _up(b), None, "gelu", torch.float32, _up(dy))
+    for g, k in ((dx, "dx"), (dw, "dw"), (db, "db")):
+        R.close(g, want[k], k)
+    with pytest.raises(RuntimeError, match="once"):
+        (dx.sum() + dw.sum() + db.sum()).backward()
+
+
+def test_gradients_accumulate_and_a_changed_input_is_noticed():
+    from fedsim_amd.functional import linear_act
+
+    x, w, b, _, dy = _case(20, 24, 16, torch.float32, 22, residual=False)
+    X, W = (t.to(DEV).requires_grad_(True) for t in (x, w))
+    for _ in range(2):
+        linear_act(X, W, activation="silu").backward(dy.to(DEV))
+    want = R.product(_up(x), _up(w), None, None, "silu", torch.float32, _up(dy))
+    for g, k in ((X.grad, "dx"), (W.grad, "dw")):
+        v, e = want[k]
+        R.close(g, (2 * v, 2 * e + 2.0 ** -23 * v.abs()), k)
+    y = linear_act(X, W)
+    with torch.no_grad():
+        W.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
