@@ -24,7 +24,6 @@ namespace {
 using namespace fedtrain;
 
 constexpr int kBlock = 256;   // elements that share a scale: 64 lanes x 4
-constexpr int kChunk = 4096;  // elements a workgroup takes: 4 waves x 4 blocks
 constexpr int kMost = 40;     // tensors a launch takes: 40 x 72 B of kernel arguments
 
 struct Tensor {
@@ -54,12 +53,6 @@ __host__ __device__ inline unsigned mix(unsigned h) {
 __device__ inline float from_bits(unsigned b) { return __builtin_bit_cast(float, b); }
 __device__ inline unsigned to_bits(float f) { return __builtin_bit_cast(unsigned, f); }
 
-// The largest of a wave's values.
-__device__ inline float wave_max(float x) {
-  for (int s = 32; s; s >>= 1) x = fmaxf(x, __shfl_xor(x, s));
-  return x;
-}
-
 // The biased exponent of a block's scale: the largest magnitude over it lies
 // between sqrt(3) 2^TOP and sqrt(3) 2^(TOP + 1), below the codes' largest.  A
 // border at 1.0 or at the largest code would be met by sums of codes.
@@ -86,96 +79,203 @@ __device__ inline Moments moments(const Batch& b, float m, float v, float g) {
   return {m * b.b1 + g * b.c1, v * b.b2 + (g * b.c2) * g};
 }
 
-__device__ inline float step_of(const Batch& b, float size, float root, float p, Moments s) {
+struct Scalars {
+  float size, root;
+  unsigned key;
+};
+
+__device__ inline float step_of(const Batch& b, const Scalars& c, float p, Moments s) {
   // the square root and the quotient of the hardware, each within one unit of
   // its last place: far below the rounding of p
-  float d = __builtin_amdgcn_sqrtf(s.v) * root + b.eps;
-  return p * b.decay - size * (s.m * __builtin_amdgcn_rcpf(d));
+  float d = __builtin_amdgcn_sqrtf(s.v) * c.root + b.eps;
+  return p * b.decay - c.size * (s.m * __builtin_amdgcn_rcpf(d));
 }
 
-template <int D, int BITS> __global__ __launch_bounds__(256) void k_adamw(Batch b) {
+template <class T, int V> struct __attribute__((aligned(V * sizeof(T)))) Vec {
+  T v[V];
+};
+
+template <class T, int V> __device__ inline Vec<T, V> get(const void* p, int64_t at) {
+  return *reinterpret_cast<const Vec<T, V>*>(static_cast<const T*>(p) + at);
+}
+template <class T, int V> __device__ inline void set(void* p, int64_t at, const Vec<T, V>& x) {
+  *reinterpret_cast<Vec<T, V>*>(static_cast<T*>(p) + at) = x;
+}
+
+// The largest of each SPAN neighbouring lanes' values.
+template <int SPAN> __device__ inline float span_max(float x) {
+#pragma unroll
+  for (int s = SPAN / 2; s; s >>= 1) x = fmaxf(x, __shfl_xor(x, s));
+  return x;
+}
+
+// The codes of V neighbouring elements of block `blk`, from its element `first`
+// on; SPAN lanes share the block, and one of them stores its scales.
+template <int V, int SPAN>
+__device__ inline void requantize(const float* m, const float* v, unsigned key, int64_t blk,
+                                  unsigned first, float* m_scale, float* v_scale,
+                                  unsigned* qm, unsigned* qv) {
+  float mm = 0, vm = 0;
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    // an infinity or NaN is that element's alone: it does not set the scale
+    mm = fmaxf(mm, fabsf(m[e]) < INFINITY ? fabsf(m[e]) : 0.0f);
+    vm = fmaxf(vm, v[e] < INFINITY ? v[e] : 0.0f);
+  }
+  const int me = scale_exponent<7>(span_max<SPAN>(mm));
+  const int ve = scale_exponent<14>(span_max<SPAN>(vm));
+  const float mi = from_bits(static_cast<unsigned>(254 - me) << 23);
+  const float vi = from_bits(static_cast<unsigned>(254 - ve) << 23);
+  const unsigned bk = mix(key + static_cast<unsigned>(blk) * 0x9E3779B9u);
+  float x[V], y[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    const unsigned h = mix(bk + (first + e) * 0x9E3779B9u);
+    x[e] = copysignf(stochastic<3, -6>(fabsf(m[e]) * mi, h & 0xFFFF), m[e]);
+    y[e] = v[e] * vi;
+    y[e] = y[e] > 0 ? fmaxf(stochastic<2, -14>(y[e], h >> 16), 0x1p-16f) : y[e];
+    // what is no number has a code of its own: NaN (m), infinity or NaN (v)
+    if (!(fabsf(m[e]) < INFINITY)) x[e] = NAN;
+    if (!(v[e] < INFINITY)) y[e] = v[e];
+  }
+#pragma unroll
+  for (int e = 0; e < V; e += 4) {
+    int a = __builtin_amdgcn_cvt_pk_fp8_f32(x[e], x[e + 1], 0, false);
+    int c = __builtin_amdgcn_cvt_pk_bf8_f32(y[e], y[e + 1], 0, false);
+    qm[e / 4] = __builtin_amdgcn_cvt_pk_fp8_f32(x[e + 2], x[e + 3], a, true);
+    qv[e / 4] = __builtin_amdgcn_cvt_pk_bf8_f32(y[e + 2], y[e + 3], c, true);
+  }
+  if ((threadIdx.x & (SPAN - 1)) == 0) {
+    *m_scale = from_bits(static_cast<unsigned>(me) << 23);
+    *v_scale = from_bits(static_cast<unsigned>(ve) << 23);
+  }
+}
+
+// V elements of a tensor from `at` on that all exist, all pointers aligned.
+template <int D, int BITS, int V>
+__device__ inline void step_wide(const Batch& b, const Scalars& c, const Tensor& t, int64_t at) {
   using T = typename Elem<D>::type;
+  const Vec<T, V> p = get<T, V>(t.t.p, at), g = get<T, V>(t.t.g, at);
+  float m[V], v[V];
+  const int64_t blk = at / kBlock;
+  if constexpr (BITS == 32) {
+    const Vec<float, V> mo = get<float, V>(t.t.m, at), vo = get<float, V>(t.t.v, at);
+#pragma unroll
+    for (int e = 0; e < V; ++e) m[e] = mo.v[e], v[e] = vo.v[e];
+  } else {
+    const Vec<unsigned, V / 4> mo = get<unsigned, V / 4>(t.t.m, at / 4);
+    const Vec<unsigned, V / 4> vo = get<unsigned, V / 4>(t.t.v, at / 4);
+    const float ms = t.t.m_scale[blk], vs = t.t.v_scale[blk];
+#pragma unroll
+    for (int e = 0; e < V; e += 4) {
+      m[e] = __builtin_amdgcn_cvt_f32_fp8(mo.v[e / 4], 0) * ms;
+      m[e + 1] = __builtin_amdgcn_cvt_f32_fp8(mo.v[e / 4], 1) * ms;
+      m[e + 2] = __builtin_amdgcn_cvt_f32_fp8(mo.v[e / 4], 2) * ms;
+      m[e + 3] = __builtin_amdgcn_cvt_f32_fp8(mo.v[e / 4], 3) * ms;
+      v[e] = __builtin_amdgcn_cvt_f32_bf8(vo.v[e / 4], 0) * vs;
+      v[e + 1] = __builtin_amdgcn_cvt_f32_bf8(vo.v[e / 4], 1) * vs;
+      v[e + 2] = __builtin_amdgcn_cvt_f32_bf8(vo.v[e / 4], 2) * vs;
+      v[e + 3] = __builtin_amdgcn_cvt_f32_bf8(vo.v[e / 4], 3) * vs;
+    }
+  }
+  Vec<T, V> out;
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    const Moments s = moments(b, m[e], v[e], Elem<D>::up(g.v[e]));
+    m[e] = s.m;
+    v[e] = s.v;
+    out.v[e] = Elem<D>::down(step_of(b, c, Elem<D>::up(p.v[e]), s));
+  }
+  set<T, V>(t.t.p, at, out);
+  if constexpr (BITS == 32) {
+    Vec<float, V> mo, vo;
+#pragma unroll
+    for (int e = 0; e < V; ++e) mo.v[e] = m[e], vo.v[e] = v[e];
+    set<float, V>(t.t.m, at, mo);
+    set<float, V>(t.t.v, at, vo);
+  } else {
+    Vec<unsigned, V / 4> qm, qv;
+    requantize<V, kBlock / V>(m, v, c.key, t.t.block0 + blk, at % kBlock, t.t.m_scale + blk,
+                              t.t.v_scale + blk, qm.v, qv.v);
+    set<unsigned, V / 4>(t.t.m, at / 4, qm);
+    set<unsigned, V / 4>(t.t.v, at / 4, qv);
+  }
+}
+
+// A wave's block at any alignment, or the short last one; 4 elements a lane.
+template <int D, int BITS>
+__device__ void step_any(const Batch& b, const Scalars& c, const Tensor& t, int64_t at) {
+  using T = typename Elem<D>::type;
+  T* P = static_cast<T*>(t.t.p);
+  const T* G = static_cast<const T*>(t.t.g);
+  const int64_t left = t.t.n - at, blk = at / kBlock;
+  const int live = left >= 4 ? 4 : left > 0 ? static_cast<int>(left) : 0;
+  float p[4], m[4], v[4];
+  const float ms = BITS == 8 ? t.t.m_scale[blk] : 1, vs = BITS == 8 ? t.t.v_scale[blk] : 1;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float g = 0;
+    p[e] = m[e] = v[e] = 0;
+    if (e < live) {
+      p[e] = Elem<D>::up(P[at + e]);
+      g = Elem<D>::up(G[at + e]);
+      if (BITS == 32) {
+        m[e] = static_cast<const float*>(t.t.m)[at + e];
+        v[e] = static_cast<const float*>(t.t.v)[at + e];
+      } else {
+        m[e] = __builtin_amdgcn_cvt_f32_fp8(static_cast<const uint8_t*>(t.t.m)[at + e], 0) * ms;
+        v[e] = __builtin_amdgcn_cvt_f32_bf8(static_cast<const uint8_t*>(t.t.v)[at + e], 0) * vs;
+      }
+    }
+    const Moments s = moments(b, m[e], v[e], g);
+    m[e] = s.m;
+    v[e] = s.v;
+    p[e] = step_of(b, c, p[e], s);
+  }
+  unsigned qm[1], qv[1];
+  if (BITS == 8)
+    requantize<4, 64>(m, v, c.key, t.t.block0 + blk, at % kBlock, t.t.m_scale + blk,
+                      t.t.v_scale + blk, qm, qv);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (e >= live) continue;
+    P[at + e] = Elem<D>::down(p[e]);
+    if (BITS == 32) {
+      static_cast<float*>(t.t.m)[at + e] = m[e];
+      static_cast<float*>(t.t.v)[at + e] = v[e];
+    } else {
+      static_cast<uint8_t*>(t.t.m)[at + e] = static_cast<uint8_t>(qm[0] >> (8 * e));
+      static_cast<uint8_t*>(t.t.v)[at + e] = static_cast<uint8_t>(qv[0] >> (8 * e));
+    }
+  }
+}
+
+// A workgroup takes `per` x 1024 elements: 1 where there is little to do, so that
+// every wave has one block and one trip to memory; 4 otherwise, with states in
+// 8 bits 16 elements a lane (whole 16-byte loads of the codes, and a block's
+// largest value among 16 lanes).
+template <int D, int BITS, int PER> __global__ __launch_bounds__(256) void k_adamw(Batch b) {
   int i = 0;
   while (i + 1 < b.count && static_cast<int>(blockIdx.x) >= b.at[i + 1].first) ++i;
   const Tensor& t = b.at[i];
-  float size = b.size, root = b.root;
-  unsigned key = b.key;
-  if (b.device) {
-    size = b.device[0];
-    root = b.device[1];
-    key = to_bits(b.device[2]);
+  const int64_t chunk = static_cast<int64_t>(blockIdx.x - t.first) * (PER * 1024);
+  Scalars c = {b.size, b.root, b.key};
+  if (b.device) c = {b.device[0], b.device[1], to_bits(b.device[2])};
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (PER == 4 && t.wide && chunk + PER * 1024 <= t.t.n) {
+    if constexpr (BITS == 8) {
+      step_wide<D, BITS, 16>(b, c, t, chunk + tid * 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) step_wide<D, BITS, 4>(b, c, t, chunk + (j * 256 + tid) * 4);
+    }
+    return;
   }
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  T* P = static_cast<T*>(t.t.p);
-  const T* G = static_cast<const T*>(t.t.g);
-  const int64_t chunk = static_cast<int64_t>(blockIdx.x - t.first) * kChunk;
-  for (int j = 0; j < kChunk / kBlock / 4; ++j) {
-    const int64_t at = chunk + (j * 4 + wave) * kBlock + lane * 4;
-    if (at - lane * 4 >= t.t.n) return;
-    const int64_t blk = at / kBlock;
-    float p[4], g[4], m[4], v[4];
-    int live = t.t.n - at >= 4 ? 4 : t.t.n - at > 0 ? static_cast<int>(t.t.n - at) : 0;
-    float ms = 1, vs = 1;
-    if (BITS == 8) {
-      ms = t.t.m_scale[blk];
-      vs = t.t.v_scale[blk];
-    }
-    for (int e = 0; e < 4; ++e) {
-      p[e] = g[e] = m[e] = v[e] = 0;
-      if (e < live) {
-        p[e] = Elem<D>::up(P[at + e]);
-        g[e] = Elem<D>::up(G[at + e]);
-        if (BITS == 32) {
-          m[e] = static_cast<const float*>(t.t.m)[at + e];
-          v[e] = static_cast<const float*>(t.t.v)[at + e];
-        } else {
-          m[e] = __builtin_amdgcn_cvt_f32_fp8(static_cast<const uint8_t*>(t.t.m)[at + e], 0) * ms;
-          v[e] = __builtin_amdgcn_cvt_f32_bf8(static_cast<const uint8_t*>(t.t.v)[at + e], 0) * vs;
-        }
-      }
-    }
-    float mm = 0, vm = 0;
-    for (int e = 0; e < 4; ++e) {
-      Moments s = moments(b, m[e], v[e], g[e]);
-      m[e] = s.m;
-      v[e] = s.v;
-      p[e] = step_of(b, size, root, p[e], s);
-      // an infinity or NaN is that element's alone: it does not set the scale
-      if (fabsf(s.m) < INFINITY) mm = fmaxf(mm, fabsf(s.m));
-      if (s.v < INFINITY) vm = fmaxf(vm, s.v);
-    }
-    uint8_t qm[4], qv[4];
-    if (BITS == 8) {
-      const int me = scale_exponent<7>(wave_max(mm)), ve = scale_exponent<14>(wave_max(vm));
-      const float mi = from_bits(static_cast<unsigned>(254 - me) << 23);
-      const float vi = from_bits(static_cast<unsigned>(254 - ve) << 23);
-      const unsigned bk = mix(key + static_cast<unsigned>(t.t.block0 + blk) * 0x9E3779B9u);
-      for (int e = 0; e < 4; ++e) {
-        const unsigned h = mix(bk + static_cast<unsigned>(lane * 4 + e) * 0x9E3779B9u);
-        float x = stochastic<3, -6>(fabsf(m[e]) * mi, h & 0xFFFF);
-        x = copysignf(x, m[e]);
-        float y = v[e] * vi;
-        y = y > 0 ? fmaxf(stochastic<2, -14>(y, h >> 16), 0x1p-16f) : y;
-        qm[e] = static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false));
-        qv[e] = static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_bf8_f32(y, y, 0, false));
-        if (!(fabsf(m[e]) < INFINITY)) qm[e] = 0x7F;
-        if (!(v[e] < INFINITY)) qv[e] = v[e] == INFINITY ? 0x7C : 0x7F;
-      }
-      if (lane == 0) {
-        t.t.m_scale[blk] = from_bits(static_cast<unsigned>(me) << 23);
-        t.t.v_scale[blk] = from_bits(static_cast<unsigned>(ve) << 23);
-      }
-    }
-    for (int e = 0; e < live; ++e) {
-      P[at + e] = Elem<D>::down(p[e]);
-      if (BITS == 32) {
-        static_cast<float*>(t.t.m)[at + e] = m[e];
-        static_cast<float*>(t.t.v)[at + e] = v[e];
-      } else {
-        static_cast<uint8_t*>(t.t.m)[at + e] = qm[e];
-        static_cast<uint8_t*>(t.t.v)[at + e] = qv[e];
-      }
-    }
+  for (int j = 0; j < PER; ++j) {
+    const int64_t first = chunk + (j * 4 + wave) * kBlock;
+    if (first >= t.t.n) return;
+    if (t.wide && first + kBlock <= t.t.n) step_wide<D, BITS, 4>(b, c, t, first + lane * 4);
+    else step_any<D, BITS>(b, c, t, first + lane * 4);
   }
 }
 
@@ -197,11 +297,16 @@ __global__ void k_adamw_scalars(double lr, double b1, double b2, unsigned seed,
   out[2] = from_bits(mix(seed ^ mix(static_cast<unsigned>(t))));
 }
 
-template <int D> void launch(int bits, unsigned grid, hipStream_t s, const Batch& b) {
-  if (bits == 32)
-    hipLaunchKernelGGL((k_adamw<D, 32>), dim3(grid), dim3(256), 0, s, b);
+template <int D, int BITS> void launch(int per, unsigned grid, hipStream_t s, const Batch& b) {
+  if (per == 1)
+    hipLaunchKernelGGL((k_adamw<D, BITS, 1>), dim3(grid), dim3(256), 0, s, b);
   else
-    hipLaunchKernelGGL((k_adamw<D, 8>), dim3(grid), dim3(256), 0, s, b);
+    hipLaunchKernelGGL((k_adamw<D, BITS, 4>), dim3(grid), dim3(256), 0, s, b);
+}
+
+template <int D> void launch(int bits, int per, unsigned grid, hipStream_t s, const Batch& b) {
+  if (bits == 32) launch<D, 32>(per, grid, s, b);
+  else launch<D, 8>(per, grid, s, b);
 }
 
 }  // namespace
@@ -218,6 +323,7 @@ extern "C" int fedtrain_adamw(int dtype, int state_bits, int64_t count,
         s->eps >= 0 && s->weight_decay >= 0))
     return FEDTRAIN_EINVAL;
   const size_t esize = dtype == FEDTRAIN_F32 ? 4 : 2, ssize = state_bits == 32 ? 4 : 1;
+  int64_t total = 0;
   for (int64_t i = 0; i < count; ++i) {
     const fedtrain_adamw_tensor& t = tensors[i];
     if (t.n < 0 || t.block0 < 0) return FEDTRAIN_EINVAL;
@@ -228,8 +334,11 @@ extern "C" int fedtrain_adamw(int dtype, int state_bits, int64_t count,
     if (state_bits == 8 &&
         (!t.m_scale || !t.v_scale || !aligned(t.m_scale, 4) || !aligned(t.v_scale, 4)))
       return FEDTRAIN_EINVAL;
-    if (t.n > static_cast<int64_t>(kChunk) << 30) return FEDTRAIN_EINVAL;
+    if (t.n > int64_t{1} << 40) return FEDTRAIN_EINVAL;
+    total += t.n;
   }
+  // below 4 workgroups of 1024 elements a compute unit the smaller ones win
+  const int per = total < 4 * 256 * 1024 ? 1 : 4;
   hipStream_t st = static_cast<hipStream_t>(stream);
   Batch b;
   b.b1 = static_cast<float>(s->beta1);
@@ -258,20 +367,19 @@ extern "C" int fedtrain_adamw(int dtype, int state_bits, int64_t count,
     for (; i < count && b.count < kMost; ++i) {
       const fedtrain_adamw_tensor& t = tensors[i];
       if (!t.n) continue;
-      const int64_t groups = (t.n + kChunk - 1) / kChunk;
+      const int64_t groups = (t.n + per * 1024 - 1) / (per * 1024);
       if (grid + groups > INT32_MAX) break;
       Tensor& at = b.at[b.count++];
       at.t = t;
       at.first = static_cast<int>(grid);
-      at.wide = aligned(t.p, 4 * esize) && aligned(t.g, 4 * esize) && aligned(t.m, 4 * ssize) &&
-                aligned(t.v, 4 * ssize);
+      at.wide = aligned(t.p, 16) && aligned(t.g, 16) && aligned(t.m, 16) && aligned(t.v, 16);
       grid += groups;
     }
     if (!b.count) break;
     const unsigned n = static_cast<unsigned>(grid);
-    if (dtype == FEDTRAIN_F32) launch<FEDTRAIN_F32>(state_bits, n, st, b);
-    else if (dtype == FEDTRAIN_BF16) launch<FEDTRAIN_BF16>(state_bits, n, st, b);
-    else launch<FEDTRAIN_F16>(state_bits, n, st, b);
+    if (dtype == FEDTRAIN_F32) launch<FEDTRAIN_F32>(state_bits, per, n, st, b);
+    else if (dtype == FEDTRAIN_BF16) launch<FEDTRAIN_BF16>(state_bits, per, n, st, b);
+    else launch<FEDTRAIN_F16>(state_bits, per, n, st, b);
     if (const int rc = launched()) return rc;
   }
   return 0;
