@@ -7,7 +7,9 @@
 //   grad weight   C = A^T B, colsum = A^T 1                A = dz, B = x
 #include "fedtrain_common.h"
 
+#include <algorithm>
 #include <climits>
+#include <cmath>
 #include <type_traits>
 
 namespace {
@@ -154,23 +156,16 @@ template <int D> __device__ inline f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// How a tile of an operand lies in LDS.  NJ: the column operand's rows are read
-// in the order that gives a lane 4 NJ neighbouring columns of C (0: in order).
-template <bool KS_, int W_, int BK_, int NJ_> struct Tile {
+template <bool KS_, int W_, int BK_> struct Tile {
   static constexpr bool KS = KS_;
-  static constexpr int W = W_, BK = BK_, NJ = NJ_;
+  static constexpr int W = W_, BK = BK_;
   static constexpr int per_line = (KS ? W : BK) / 8;
   static constexpr int chunks = W * BK / 8;
   static constexpr int bytes = chunks * 16;  // of one plane
 
   static __device__ int swizzle(int line) {
-    if constexpr (KS) {
-      return (((line & 3) | ((line >> 3) & 3) << 2) & (W / 16 - 1)) << 1;
-    } else {
-      const int high = NJ == 0 ? 2 : NJ == 1 ? 2 : NJ == 2 ? 3 : 4;  // of the next 4 lanes' rows
-      if constexpr (BK == 64) return (line & 3) | ((line >> high) & 1) << 2;
-      return ((line >> 1) & 1) | ((line >> high) & 1) << 1;
-    }
+    if constexpr (KS) return (((line & 3) | ((line >> 3) & 3) << 2) & (W / 16 - 1)) << 1;
+    return BK == 64 ? line & 7 : (line >> 1) & 3;
   }
   static __device__ int at(int line, int chunk) {
     return (line * per_line + (chunk ^ swizzle(line))) * 16;
@@ -189,23 +184,26 @@ template <bool KS_, int W_, int BK_, int NJ_> struct Tile {
       }
       return __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
     } else {
-      const int row = row0 + (NJ ? (r >> 2) * (4 * NJ) + t * 4 + (r & 3) : t * 16 + r);
-      return *reinterpret_cast<const s16x8*>(base + at(row, kk * 4 + q));
+      return *reinterpret_cast<const s16x8*>(base + at(row0 + t * 16 + r, kk * 4 + q));
     }
   }
 };
 
-// x's three bf16 parts, in the high halves.  An infinity or NaN is its first
-// part alone; true for those.  (Parts below 2^-126 may be lost.)
+// x's three bf16 parts, in the high halves, with garbage below them.  True for an
+// infinity or NaN, whose parts are wrong.  (Parts below 2^-126 may be lost.)
 __device__ inline bool split3(float x, unsigned& h, unsigned& m, unsigned& l) {
-  const unsigned b = __builtin_bit_cast(unsigned, x);
-  h = b & 0xFFFF0000u;
-  const bool odd = (b & 0x7F800000u) == 0x7F800000u;
-  if (odd && (b & 0xFFFFu)) h |= 0x10000u;  // a NaN stays one
-  const float r = odd ? 0.0f : x - __builtin_bit_cast(float, h);
-  m = __builtin_bit_cast(unsigned, r) & 0xFFFF0000u;
-  l = __builtin_bit_cast(unsigned, r - __builtin_bit_cast(float, m)) & 0xFFFF0000u;
-  return odd;
+  h = __builtin_bit_cast(unsigned, x);
+  const float r = x - __builtin_bit_cast(float, h & 0xFFFF0000u);
+  m = __builtin_bit_cast(unsigned, r);
+  l = __builtin_bit_cast(unsigned, r - __builtin_bit_cast(float, m & 0xFFFF0000u));
+  return r != r;
+}
+
+// The same with an infinity or NaN as its first part alone.
+__device__ inline void split3_any(float x, unsigned& h, unsigned& m, unsigned& l) {
+  if (!split3(x, h, m, l)) return;
+  m = l = 0;
+  if (x != x) h |= 0x10000u;  // a NaN stays one
 }
 
 // The value that three parts stand for.
@@ -227,6 +225,8 @@ template <int D, class L, int THREADS, bool DIRECT> struct Loader {
   int64_t ld;
   int rows;
   u32x4 held[DIRECT ? 1 : N][R];
+  const T* from[DIRECT ? 1 : N];  // the chunk's place in the tile under way
+  int some[DIRECT ? 1 : N];       // its values that exist (KS), or whether its row does (KC)
   unsigned offset[DIRECT ? N : 1];
 
   __device__ void init(const void* p, int64_t ld_, int64_t row0, int64_t rows_, int tid) {
@@ -247,6 +247,7 @@ template <int D, class L, int THREADS, bool DIRECT> struct Loader {
   // DIRECT: memory to LDS without registers.  A lane outside the operand asks
   // for an offset past the descriptor's range, which stores zeros.
   __device__ void issue(int64_t k, int64_t k1, char* to, int tid) const {
+    if (k > k1) k = k1;  // past the end every lane asks for zeros
     const int64_t first = L::KS ? k * ld : k;
     auto d = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base + first), 0, 0x7FFFFFFF,
                                                0x00027000);
@@ -265,76 +266,99 @@ template <int D, class L, int THREADS, bool DIRECT> struct Loader {
     }
   }
 
-  // through registers: any alignment, any length
-  __device__ void load(int64_t k, int64_t k1, int tid) {
+  // through registers: any alignment, any length.  For steps of BK from k on.
+  __device__ void begin(int64_t k, int tid) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int q = tid + i * THREADS, line = q / L::per_line;
       const int c = (q % L::per_line) ^ L::swizzle(line);
-      const int row = L::KS ? c * 8 : line;
-      const int64_t kk = k + (L::KS ? line : c * 8);
-      const T* p = base + (L::KS ? kk * ld + row : row * ld + kk);
-      int n = L::KS ? (kk < k1 ? rows - row : 0)
-                    : (row < rows ? static_cast<int>(k1 - kk < 8 ? k1 - kk : 8) : 0);
-      if (n >= 8) {
-        __builtin_memcpy(&held[i][0], p, 16 * R);
-      } else {
-        T v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = e < n ? p[e] : Elem<D>::down(0);
-        __builtin_memcpy(&held[i][0], v, 16 * R);
-      }
+      from[i] = base + (L::KS ? (k + line) * ld + c * 8 : line * ld + k + c * 8);
+      some[i] = L::KS ? rows - c * 8 : line < rows ? 8 : 0;
     }
   }
 
-  // f32: *odd becomes 1 where an infinity or NaN was met
-  __device__ void store(char* to, int tid, int* odd) const {
-    bool met = false;
+  // the next tile, of which `left` k exist
+  __device__ void load(int64_t left, int tid) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      char* p = to + (tid + i * THREADS) * 16;
-      if constexpr (D != FEDTRAIN_F32) {
-        *reinterpret_cast<u32x4*>(p) = held[i][0];
-      } else {
-        u32x4 out[3];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          unsigned h[2], m[2], l[2];
-#pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            const int n = e * 2 + s;
-            const unsigned bits = held[i][n / 4][n % 4];
-            met |= split3(__builtin_bit_cast(float, bits), h[s], m[s], l[s]);
-          }
-          out[0][e] = __builtin_amdgcn_perm(h[1], h[0], 0x07060302);
-          out[1][e] = __builtin_amdgcn_perm(m[1], m[0], 0x07060302);
-          out[2][e] = __builtin_amdgcn_perm(l[1], l[0], 0x07060302);
-        }
-#pragma unroll
-        for (int e = 0; e < 3; ++e) *reinterpret_cast<u32x4*>(p + e * L::bytes) = out[e];
+      int n = some[i];
+      if (left < L::BK) {
+        const int q = tid + i * THREADS, line = q / L::per_line;
+        const int c = (q % L::per_line) ^ L::swizzle(line);
+        const int more = static_cast<int>(left) - (L::KS ? line : c * 8);
+        n = L::KS ? (more > 0 ? n : 0) : (more < n ? more : n);
       }
+      if (n >= 8) {
+        __builtin_memcpy(&held[i][0], from[i], 16 * R);
+      } else {
+        T v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = e < n ? from[i][e] : Elem<D>::down(0);
+        __builtin_memcpy(&held[i][0], v, 16 * R);
+      }
+      from[i] += L::KS ? L::BK * ld : L::BK;
     }
-    if (D == FEDTRAIN_F32 && met) *odd = 1;
+  }
+
+  // chunk i to its place; f32: true where an infinity or NaN was met, whose parts
+  // are right with ANY alone
+  template <bool ANY> __device__ bool put(int i, char* to, int tid) const {
+    char* p = to + (tid + i * THREADS) * 16;
+    bool met = false;
+    if constexpr (D != FEDTRAIN_F32) {
+      *reinterpret_cast<u32x4*>(p) = held[i][0];
+    } else {
+      u32x4 out[3];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        unsigned h[2], m[2], l[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const int n = e * 2 + s;
+          const unsigned bits = held[i][n / 4][n % 4];
+          const float x = __builtin_bit_cast(float, bits);
+          if (ANY) split3_any(x, h[s], m[s], l[s]);
+          else met |= split3(x, h[s], m[s], l[s]);
+        }
+        out[0][e] = __builtin_amdgcn_perm(h[1], h[0], 0x07060302);
+        out[1][e] = __builtin_amdgcn_perm(m[1], m[0], 0x07060302);
+        out[2][e] = __builtin_amdgcn_perm(l[1], l[0], 0x07060302);
+      }
+#pragma unroll
+      for (int e = 0; e < 3; ++e) *reinterpret_cast<u32x4*>(p + e * L::bytes) = out[e];
+    }
+    return met;
+  }
+  template <bool ANY> __device__ bool put_all(char* to, int tid) const {
+    bool met = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i) met |= put<ANY>(i, to, tid);
+    return met;
   }
 };
 
 // The shape of a workgroup: MW x NW waves, each with MI x NI tiles of 16 x 16.
-template <int MW_, int NW_, int MI_, int NI_, int BK_> struct Shape {
-  static constexpr int MW = MW_, NW = NW_, MI = MI_, NI = NI_, BK = BK_;
+// PASS of the MI at a time are written to C.  STAGES of tiles in LDS: 1 where they
+// come through registers, more where they come without.
+template <int MW_, int NW_, int MI_, int NI_, int BK_, int PASS_, int STAGES_ = 1> struct Shape {
+  static constexpr bool DIRECT = STAGES_ > 1;
+  static constexpr int STAGES = STAGES_;
+  static constexpr int MW = MW_, NW = NW_, MI = MI_, NI = NI_, BK = BK_, PASS = PASS_;
   static constexpr int BM = MW * MI * 16, BN = NW * NI * 16, THREADS = MW * NW * 64;
 };
 
 // Workgroups go to the 8 dies in turn.  Each die gets a contiguous part of the
-// tiles, in bands of 8 rows of tiles, so that what its workgroups read at a time
-// is shared in its own L2.
-__device__ inline void place(int64_t tiles_m, int64_t tiles_n, int64_t& tm, int64_t& tn) {
+// tiles, in bands of `high` rows of tiles, so that what its workgroups read at a
+// time is shared in its own L2.
+__device__ inline void place(int64_t tiles_m, int64_t tiles_n, int high, int64_t& tm,
+                             int64_t& tn) {
   const int64_t total = tiles_m * tiles_n, id = blockIdx.x;
   const int64_t share = total / 8, more = total % 8, die = id % 8;
   const int64_t t = die * share + (die < more ? die : more) + id / 8;
-  const int64_t band = t / (8 * tiles_n), in = t - band * 8 * tiles_n;
-  const int64_t height = tiles_m - band * 8 < 8 ? tiles_m - band * 8 : 8;
+  const int64_t band = t / (high * tiles_n), in = t - band * high * tiles_n;
+  const int64_t height = tiles_m - band * high < high ? tiles_m - band * high : high;
   tn = in / height;
-  tm = band * 8 + in % height;
+  tm = band * high + in % height;
 }
 
 __device__ inline void arrive() {
@@ -346,91 +370,93 @@ template <int N> __device__ inline void wait_loads() {
 
 struct Plan {
   int64_t tiles_m, tiles_n;  // tiles_m: of one group (grad weight), or slots
+  int high;                  // rows of tiles in a band, see place()
   int splits;                // parts of k; over 1, C is f32 partial sums in the workspace
-  int wide;                  // 1: four neighbouring values of every operand of C at a time
+  int wide;                  // 1: eight neighbouring values of C's operands are 16-byte aligned
 };
 
 // ---------------------------------------------------------------------------
 // what becomes of the sums
 // ---------------------------------------------------------------------------
-template <class T> struct __attribute__((aligned(4 * sizeof(T)))) Four {
-  T v[4];
+// Eight neighbouring values in memory, as one or two accesses of 16 bytes; n of
+// them where they are not `wide`.
+template <class T> struct __attribute__((aligned(16))) Eight {
+  T v[8];
 };
 
-template <int D> __device__ inline void read4(const void* p, int64_t at, int n, bool wide,
+template <int D> __device__ inline void read8(const void* p, int64_t at, int n, bool wide,
                                               float* to) {
   using T = typename Elem<D>::type;
   const T* x = static_cast<const T*>(p) + at;
   if (wide) {
-    const Four<T> f = *reinterpret_cast<const Four<T>*>(x);
+    const Eight<T> f = *reinterpret_cast<const Eight<T>*>(x);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) to[e] = Elem<D>::up(f.v[e]);
+    for (int e = 0; e < 8; ++e) to[e] = Elem<D>::up(f.v[e]);
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) to[e] = e < n ? Elem<D>::up(x[e]) : 0.0f;
+    for (int e = 0; e < 8; ++e) to[e] = e < n ? Elem<D>::up(x[e]) : 0.0f;
   }
 }
 
-template <int D> __device__ inline void write4(void* p, int64_t at, int n, bool wide,
+template <int D> __device__ inline void write8(void* p, int64_t at, int n, bool wide,
                                                const float* v) {
   using T = typename Elem<D>::type;
   T* x = static_cast<T*>(p) + at;
   if (wide) {
-    Four<T> f;
+    Eight<T> f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) f.v[e] = Elem<D>::down(v[e]);
-    *reinterpret_cast<Four<T>*>(x) = f;
+    for (int e = 0; e < 8; ++e) f.v[e] = Elem<D>::down(v[e]);
+    *reinterpret_cast<Eight<T>*>(x) = f;
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int e = 0; e < 8; ++e)
       if (e < n) x[e] = Elem<D>::down(v[e]);
   }
 }
 
-// n <= 4 neighbouring sums of a row of C, to their end
+// n neighbouring sums of a row of C (8, where wide), to their end
 template <int D, int FORM, int ACT>
 __device__ inline void put(const Args& a, int group, int64_t row, int64_t col, int n, bool wide,
                            float* v) {
   if constexpr (FORM == FEDTRAIN_FORWARD) {
     if (group >= 0) {
       if (a.bias) {
-        float b[4];
-        read4<D>(a.bias, group * a.bias_group + col, n, wide, b);
+        float b[8];
+        read8<D>(a.bias, group * a.bias_group + col, n, wide, b);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] += b[e];
+        for (int e = 0; e < 8; ++e) v[e] += b[e];
       }
-      if (a.z) write4<D>(a.z, row * a.ldz + col, n, wide, v);
+      if (a.z) write8<D>(a.z, row * a.ldz + col, n, wide, v);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = act_value<D, ACT>(v[e]);
+      for (int e = 0; e < 8; ++e) v[e] = act_value<D, ACT>(v[e]);
     } else if (a.z) {
-      write4<D>(a.z, row * a.ldz + col, n, wide, v);
+      write8<D>(a.z, row * a.ldz + col, n, wide, v);
     }
     if (a.res) {
-      float r[4];
-      read4<D>(a.res, row * a.ldr + col, n, wide, r);
+      float r[8];
+      read8<D>(a.res, row * a.ldr + col, n, wide, r);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += r[e];
+      for (int e = 0; e < 8; ++e) v[e] += r[e];
     }
   }
   const int64_t first = FORM == FEDTRAIN_GRAD_WEIGHT ? group * a.c_group : 0;
-  write4<D>(a.c, first + row * a.ldc + col, n, wide, v);
+  write8<D>(a.c, first + row * a.ldc + col, n, wide, v);
 }
-
-template <int D, int FORM, class S, bool DIRECT>
-__global__ __launch_bounds__(S::THREADS) void k_product(Args a, Plan plan) {
+template <int D, int FORM, class S> __global__ __launch_bounds__(S::THREADS, 2)
+void k_product(Args a, Plan plan) {
 #ifdef __HIP_DEVICE_COMPILE__  // the host's pass needs the name alone
   using T = typename Elem<D>::type;
   constexpr bool WEIGHT = FORM == FEDTRAIN_GRAD_WEIGHT;
   constexpr int PLANES = D == FEDTRAIN_F32 ? 3 : 1;
-  using LA = Tile<WEIGHT, S::BM, S::BK, 0>;
-  using LB = Tile<FORM != FEDTRAIN_FORWARD, S::BN, S::BK, FORM == FEDTRAIN_FORWARD ? S::NI : 0>;
+  using LA = Tile<WEIGHT, S::BM, S::BK>;
+  using LB = Tile<FORM != FEDTRAIN_FORWARD, S::BN, S::BK>;
   constexpr int STAGE = PLANES * (LA::bytes + LB::bytes);
   extern __shared__ __attribute__((aligned(1024))) char lds[];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int wm = wave / S::NW * (S::MI * 16), wn = wave % S::NW * (S::NI * 16);
   int64_t slot, tn;
-  place(plan.tiles_m * (WEIGHT && a.groups ? a.groups : 1), plan.tiles_n, slot, tn);
+  place(plan.tiles_m * (WEIGHT && a.groups ? a.groups : 1), plan.tiles_n, plan.high, slot, tn);
   const int64_t col0 = tn * S::BN;
   int64_t row0, rows, k0 = 0, k1 = a.k;
   int group = 0;
@@ -460,181 +486,274 @@ __global__ __launch_bounds__(S::THREADS) void k_product(Args a, Plan plan) {
   const T* B = static_cast<const T*>(a.b);
   if (!WEIGHT && group > 0) B += group * a.b_group;
 
-  Loader<D, LA, S::THREADS, DIRECT> la;
-  Loader<D, LB, S::THREADS, DIRECT> lb;
+  Loader<D, LA, S::THREADS, S::DIRECT> la;
+  Loader<D, LB, S::THREADS, S::DIRECT> lb;
   la.init(a.a, a.lda, row0, rows, tid);
   lb.init(B, a.ldb, col0, cols, tid);
 
   f32x4 acc[S::MI][S::NI] = {};
-  f32x4 sum[S::MI] = {};
+  // sums of A's columns: the waves of C's first columns multiply by ones
+  f32x4 sum[WEIGHT ? S::MI : 1] = {};
   const bool want_sum = WEIGHT && a.colsum && col0 == 0 && wn == 0;
+  s16x8 one;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) one[e] = D == FEDTRAIN_F16 ? 0x3C00 : 0x3F80;
+  // what of the wave's rows exists; a wave without any has nothing to multiply
+  const int mine_rows = static_cast<int>(rows) - wm;
+  const bool live = mine_rows > 0 && (wn < cols || want_sum);
 
-  int* odd = reinterpret_cast<int*>(lds + (DIRECT ? 2 : 1) * STAGE);
-  auto compute = [&](const char* at) {
-    const char* pa = at;
-    const char* pb = at + PLANES * LA::bytes;
+  // the columns of C go to the rows of the unit's result: a lane gets 4
+  // neighbouring columns of a row of C
+  if constexpr (S::DIRECT) {
+    // Two stages in LDS, and a k step's fragments in registers ahead of their
+    // use: a stage is read while the one before is multiplied, so there is one
+    // barrier for each stage, and it is met with products still to do.
+    static_assert(S::BK == 64 && S::STAGES == 2, "two k steps, two stages");
+    struct Fragments {
+      s16x8 a[S::MI], b[S::NI];
+    };
+    auto read = [&](Fragments& f, const char* at, int kk) {
 #pragma unroll
-    for (int kk = 0; kk < S::BK / 32; ++kk) {
-      s16x8 fb[S::NI][PLANES];
+      for (int j = 0; j < S::NI; ++j) f.b[j] = LB::fragment(at + LA::bytes, wn, j, kk, lane);
 #pragma unroll
-      for (int j = 0; j < S::NI; ++j)
-#pragma unroll
-        for (int p = 0; p < PLANES; ++p)
-          fb[j][p] = LB::fragment(pb + p * LB::bytes, wn, j, kk, lane);
+      for (int i = 0; i < S::MI; ++i) f.a[i] = LA::fragment(at, wm, i, kk, lane);
+    };
+    // a step's products, and between them the next step's reads
+    auto multiply = [&](const Fragments& f, Fragments& other, const char* at, int kk,
+                        auto with_sum) {
+      if (!live) return;
+      read(other, at, kk);
 #pragma unroll
       for (int i = 0; i < S::MI; ++i) {
-        s16x8 fa[PLANES];
 #pragma unroll
-        for (int p = 0; p < PLANES; ++p)
-          fa[p] = LA::fragment(pa + p * LA::bytes, wm, i, kk, lane);
-        if constexpr (D == FEDTRAIN_F32) {
-          // an infinity times a part that is 0 would be NaN: with one about, the
-          // f32 unit takes the values as they were
-          if (*odd) {
-#pragma unroll 1
-            for (int e = 0; e < 8; ++e) {
-              const float x = joined(fa[0][e], fa[1][e], fa[2][e]);
-#pragma unroll
-              for (int j = 0; j < S::NI; ++j)
-                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                    joined(fb[j][0][e], fb[j][1][e], fb[j][2][e]), x, acc[i][j], 0, 0, 0);
-              if (want_sum) sum[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(1.0f, x, sum[i], 0, 0, 0);
-            }
-            continue;
-          }
-        }
-        // the columns go to the rows of the unit's result: a lane gets 4
-        // neighbouring columns
-#pragma unroll
-        for (int p = PLANES - 1; p >= 0; --p)
-#pragma unroll
-          for (int s = 0; s <= p; ++s)
-#pragma unroll
-            for (int j = 0; j < S::NI; ++j)
-              acc[i][j] = mfma<D>(fb[j][s], fa[p - s], acc[i][j]);
-        if (want_sum) {
-          s16x8 one;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) one[e] = D == FEDTRAIN_F16 ? 0x3C00 : 0x3F80;
-#pragma unroll
-          for (int p = PLANES - 1; p >= 0; --p) sum[i] = mfma<D>(one, fa[p], sum[i]);
-        }
+        for (int j = 0; j < S::NI; ++j) acc[i][j] = mfma<D>(f.b[j], f.a[i], acc[i][j]);
+        if constexpr (decltype(with_sum)::value) sum[i] = mfma<D>(one, f.a[i], sum[i]);
       }
-    }
-  };
-
-  if constexpr (DIRECT) {
+      constexpr int READS = S::NI * (LB::KS ? 2 : 1) + S::MI * (LA::KS ? 2 : 1);
+      constexpr int EACH = S::MI * S::NI / READS > 0 ? S::MI * S::NI / READS : 1;
+#pragma unroll
+      for (int r = 0; r < READS; ++r) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);   // an LDS read
+        __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);  // products
+      }
+    };
+    auto issue = [&](int64_t k, char* to) {
+      la.issue(k, k1, to, tid);
+      lb.issue(k, k1, to + LA::bytes, tid);
+    };
     constexpr int LOADS = LA::chunks / S::THREADS + LB::chunks / S::THREADS;
-    if (k0 < k1) {
-      la.issue(k0, k1, lds, tid);
-      lb.issue(k0, k1, lds + LA::bytes, tid);
-    }
-    int turn = 0;
-    for (int64_t k = k0; k < k1; k += S::BK, turn ^= 1) {
-      if (k + S::BK < k1) {
-        char* next = lds + (turn ^ 1) * STAGE;
-        la.issue(k + S::BK, k1, next, tid);
-        lb.issue(k + S::BK, k1, next + LA::bytes, tid);
-        wait_loads<LOADS>();
-      } else {
+    auto loop = [&](auto with_sum) {
+      Fragments f[2];
+      issue(k0, lds);
+      issue(k0 + S::BK, lds + STAGE);
+      wait_loads<LOADS>();
+      arrive();
+      if (live) read(f[0], lds, 0);
+      int turn = 0;
+      for (int64_t k = k0; k < k1; k += S::BK, turn ^= 1) {
+        char* now = lds + turn * STAGE;
+        multiply(f[0], f[1], now, 1, with_sum);
         wait_loads<0>();
+        arrive();
+        if (k + 2 * S::BK < k1) issue(k + 2 * S::BK, now);
+        multiply(f[1], f[0], lds + (turn ^ 1) * STAGE, 0, with_sum);
       }
-      arrive();
-      compute(lds + turn * STAGE);
-      arrive();
+    };
+    if (k0 < k1) {
+      if constexpr (WEIGHT) {
+        // one of the two for the whole workgroup: both have its barriers
+        if (a.colsum && col0 == 0) loop(std::true_type());
+        else loop(std::false_type());
+      } else {
+        loop(std::false_type());
+      }
     }
   } else {
+    int* odd = reinterpret_cast<int*>(lds + STAGE);
     if (D == FEDTRAIN_F32) {
       if (tid == 0) *odd = 0;
       __syncthreads();
     }
-    if (k0 < k1) {
-      la.load(k0, k1, tid);
-      lb.load(k0, k1, tid);
-    }
-    for (int64_t k = k0; k < k1; k += S::BK) {
-      la.store(lds, tid, odd);
-      lb.store(lds + PLANES * LA::bytes, tid, odd);
-      __syncthreads();
-      if (k + S::BK < k1) {
-        la.load(k + S::BK, k1, tid);
-        lb.load(k + S::BK, k1, tid);
+    // the loaded tile to LDS; an infinity or NaN leaves its mark
+    auto fill = [&](char* to) {
+      bool met = la.template put_all<false>(to, tid);
+      met |= lb.template put_all<false>(to + PLANES * LA::bytes, tid);
+      return met;
+    };
+    auto fill_any = [&](char* to) {
+      la.template put_all<true>(to, tid);
+      lb.template put_all<true>(to + PLANES * LA::bytes, tid);
+      *odd = 1;
+    };
+    auto multiply = [&](const char* pa, auto with_sum) {
+      const char* pb = pa + PLANES * LA::bytes;
+#pragma unroll
+      for (int kk = 0; kk < S::BK / 32; ++kk) {
+        s16x8 fb[S::NI][PLANES];
+#pragma unroll
+        for (int j = 0; j < S::NI; ++j)
+#pragma unroll
+          for (int p = 0; p < PLANES; ++p)
+            fb[j][p] = LB::fragment(pb + p * LB::bytes, wn, j, kk, lane);
+#pragma unroll
+        for (int i = 0; i < S::MI; ++i) {
+          if (S::MW == 1 && i * 16 >= mine_rows) continue;
+          s16x8 fa[PLANES];
+#pragma unroll
+          for (int p = 0; p < PLANES; ++p)
+            fa[p] = LA::fragment(pa + p * LA::bytes, wm, i, kk, lane);
+#pragma unroll
+          for (int p = PLANES - 1; p >= 0; --p) {
+#pragma unroll
+            for (int s = 0; s <= p; ++s)
+#pragma unroll
+              for (int j = 0; j < S::NI; ++j)
+                acc[i][j] = mfma<D>(fb[j][s], fa[p - s], acc[i][j]);
+            if constexpr (decltype(with_sum)::value) sum[i] = mfma<D>(one, fa[p], sum[i]);
+          }
+        }
       }
-      compute(lds);
-      __syncthreads();
+    };
+    // an infinity times a part that is 0 would be NaN: with one about, the f32
+    // unit takes the values as they were
+    auto multiply_any = [&](const char* pa, auto with_sum) {
+      const char* pb = pa + PLANES * LA::bytes;
+      if constexpr (D == FEDTRAIN_F32) {
+#pragma unroll
+        for (int i = 0; i < S::MI; ++i) {
+          s16x8 x[3];
+          for (int p = 0; p < 3; ++p) x[p] = LA::fragment(pa + p * LA::bytes, wm, i, 0, lane);
+#pragma unroll
+          for (int j = 0; j < S::NI; ++j) {
+            s16x8 w[3];
+            for (int p = 0; p < 3; ++p) w[p] = LB::fragment(pb + p * LB::bytes, wn, j, 0, lane);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                  joined(w[0][e], w[1][e], w[2][e]), joined(x[0][e], x[1][e], x[2][e]),
+                  acc[i][j], 0, 0, 0);
+          }
+          if constexpr (decltype(with_sum)::value) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              sum[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                  1.0f, joined(x[0][e], x[1][e], x[2][e]), sum[i], 0, 0, 0);
+          }
+        }
+      }
+    };
+    auto load = [&](int64_t left) {
+      la.load(left, tid);
+      lb.load(left, tid);
+    };
+    auto loop = [&](auto with_sum) {
+      la.begin(k0, tid);
+      lb.begin(k0, tid);
+      load(k1 - k0);
+      for (int64_t k = k0; k < k1; k += S::BK) {
+        if (fill(lds)) fill_any(lds);
+        __syncthreads();
+        if (k + S::BK < k1) load(k1 - k - S::BK);
+        const bool plain = D != FEDTRAIN_F32 || !__builtin_amdgcn_readfirstlane(*odd);
+        if (live && plain) multiply(lds, with_sum);
+        if (live && !plain) multiply_any(lds, with_sum);
+        __syncthreads();
+      }
+    };
+    if (k0 < k1) {
+      if constexpr (WEIGHT) {
+        if (a.colsum && col0 == 0) loop(std::true_type());
+        else loop(std::false_type());
+      } else {
+        loop(std::false_type());
+      }
     }
   }
 
-  // a lane holds the columns of one row: 4 NI neighbours (forward), or 4 in each
-  // tile
-  const int r16 = lane & 15, q = lane >> 4;
-  auto column = [&](int j) { return wn + (LB::NJ ? q * 4 * S::NI + j * 4 : j * 16 + q * 4); };
-  if (plan.splits > 1) {
-    const int64_t width = (a.n + 3) / 4 * 4 + (a.colsum ? 4 : 0);
+  const int64_t width = (a.n + 7) / 8 * 8 + (a.colsum ? 8 : 0);  // of a row of partial sums
+  float* partial = static_cast<float*>(a.workspace) +
+                   (static_cast<int64_t>(blockIdx.y) * a.m + row0) * width;
+  arrive();  // LDS is free
+  if constexpr (WEIGHT) {
+    if (want_sum && lane < 16) {
 #pragma unroll
-    for (int i = 0; i < S::MI; ++i) {
-      const int r = wm + i * 16 + r16;
-      if (r >= rows) continue;
-      float* P = static_cast<float*>(a.workspace) +
-                 (static_cast<int64_t>(blockIdx.y) * a.m + row0 + r) * width;
-#pragma unroll
-      for (int j = 0; j < S::NI; ++j)
-        if (column(j) < cols) *reinterpret_cast<f32x4*>(P + col0 + column(j)) = acc[i][j];
-      if (want_sum && q == 0) P[width - 4] = sum[i][0];
-    }
-    return;
-  }
-  if (want_sum && q == 0) {
-#pragma unroll
-    for (int i = 0; i < S::MI; ++i) {
-      const int r = wm + i * 16 + r16;
-      if (r < rows)
-        static_cast<T*>(a.colsum)[group * a.colsum_group + row0 + r] = Elem<D>::down(sum[i][0]);
-    }
-  }
-  if (WEIGHT && !a.c) return;
-  by_act(FORM == FEDTRAIN_FORWARD ? a.act : 0, [&](auto act) {
-#pragma unroll
-    for (int i = 0; i < S::MI; ++i) {
-      const int r = wm + i * 16 + r16;
-      if (r >= rows) continue;
-#pragma unroll
-      for (int j = 0; j < S::NI; ++j) {
-        const int c = column(j), n = static_cast<int>(cols) - c;
-        if (n <= 0) continue;
-        float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-        put<D, FORM, decltype(act)::value>(a, group, row0 + r, col0 + c, n, plan.wide && n >= 4,
-                                           v);
+      for (int i = 0; i < S::MI; ++i) {
+        const int r = wm + i * 16 + lane;
+        if (r >= rows) continue;
+        if (plan.splits > 1) partial[r * width + width - 8] = sum[i][0];
+        else
+          static_cast<T*>(a.colsum)[group * a.colsum_group + row0 + r] =
+              Elem<D>::down(sum[i][0]);
       }
     }
-  });
+    if (!a.c) return;
+  }
+
+  // The sums go through the wave's own part of LDS, some rows at a time, and come
+  // back as eight neighbours of a row, rows one after another: whole lines of
+  // memory, and one copy of the code that follows.
+  constexpr int LINE = S::NI * 16, EIGHTS = S::NI * 2, FIT = S::PASS;
+  f32x4* mine = reinterpret_cast<f32x4*>(lds) + wave * (FIT * 16 * LINE / 4);
+  auto spot = [](int row, int four) { return row * (LINE / 4) + (four ^ (row & (LINE / 4 - 1))); };
+#pragma unroll
+  for (int i0 = 0; i0 < S::MI; i0 += FIT) {
+#pragma unroll
+    for (int i = 0; i < FIT; ++i)
+#pragma unroll
+      for (int j = 0; j < S::NI; ++j)
+        mine[spot(i * 16 + (lane & 15), j * 4 + (lane >> 4))] = acc[i0 + i][j];
+    by_act(FORM == FEDTRAIN_FORWARD ? a.act : 0, [&](auto act) {
+#pragma unroll 2
+      for (int u = lane; u < FIT * 16 * EIGHTS; u += 64) {
+        const int row = u / EIGHTS, c8 = u % EIGHTS;
+        const f32x4 lo = mine[spot(row, c8 * 2)], hi = mine[spot(row, c8 * 2 + 1)];
+        float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        const int r = wm + i0 * 16 + row, c = wn + c8 * 8, n = static_cast<int>(cols) - c;
+        if (r >= rows || n <= 0) continue;
+        if (plan.splits > 1) {
+          Eight<float> f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f.v[e] = v[e];
+          *reinterpret_cast<Eight<float>*>(partial + r * width + col0 + c) = f;
+        } else {
+          put<D, FORM, decltype(act)::value>(a, group, row0 + r, col0 + c, n,
+                                             plan.wide && n >= 8, v);
+        }
+      }
+    });
+  }
 #endif
 }
 
-// The parts of k added up in their order, for four columns a thread.
+// The parts of k added up in their order, for eight columns a thread.
 template <int D, int FORM> __global__ __launch_bounds__(256) void k_join(Args a, Plan plan) {
   using T = typename Elem<D>::type;
-  const int64_t width = (a.n + 3) / 4 * 4 + (a.colsum ? 4 : 0), per = width / 4;
+  const int64_t width = (a.n + 7) / 8 * 8 + (a.colsum ? 8 : 0), per = width / 8;
   const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (id >= a.m * per) return;
-  const int64_t row = id / per, col = id % per * 4;
+  const int64_t row = id / per, col = id % per * 8;
   const float* P = static_cast<const float*>(a.workspace) + row * width + col;
-  f32x4 x = {0, 0, 0, 0};
-  for (int s = 0; s < plan.splits; ++s) x += *reinterpret_cast<const f32x4*>(P + s * a.m * width);
+  float v[8] = {};
+#pragma unroll 4
+  for (int s = 0; s < plan.splits; ++s) {
+    const Eight<float> f = *reinterpret_cast<const Eight<float>*>(P + s * a.m * width);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += f.v[e];
+  }
   if (col >= a.n) {
-    if (a.colsum) static_cast<T*>(a.colsum)[row] = Elem<D>::down(x[0]);
+    if (a.colsum) static_cast<T*>(a.colsum)[row] = Elem<D>::down(v[0]);
     return;
   }
   if (FORM == FEDTRAIN_GRAD_WEIGHT && !a.c) return;
   int group = 0;
   if (FORM != FEDTRAIN_GRAD_WEIGHT && a.groups) {
     group = group_of(a, row);
-    if (group < 0) x = f32x4{0, 0, 0, 0};
+    if (group < 0)
+      for (int e = 0; e < 8; ++e) v[e] = 0;
   }
-  const int n = static_cast<int>(a.n - col < 4 ? a.n - col : 4);
-  float v[4] = {x[0], x[1], x[2], x[3]};
+  const int n = static_cast<int>(a.n - col < 8 ? a.n - col : 8);
   by_act(FORM == FEDTRAIN_FORWARD ? a.act : 0, [&](auto act) {
-    put<D, FORM, decltype(act)::value>(a, group, row, col, n, plan.wide && n >= 4, v);
+    put<D, FORM, decltype(act)::value>(a, group, row, col, n, plan.wide && n >= 8, v);
   });
 }
 
@@ -710,11 +829,12 @@ bool in_eights(const Args& a) {
          a.lda < (1 << 21) && a.ldb < (1 << 21);
 }
 
-bool in_fours(const Args& a) {
-  const size_t size = a.dtype == FEDTRAIN_F32 ? 16 : 8;
-  return aligned(a.c, size) && aligned(a.z, size) && aligned(a.res, size) &&
-         aligned(a.bias, size) && a.ldc % 4 == 0 && a.c_group % 4 == 0 &&
-         (!a.z || a.ldz % 4 == 0) && (!a.res || a.ldr % 4 == 0) && a.bias_group % 4 == 0;
+// Whether eight neighbours of C and what goes into it are 16-byte accesses.
+bool out_in_eights(const Args& a) {
+  const int64_t n = a.dtype == FEDTRAIN_F32 ? 4 : 8;
+  return aligned(a.c, 16) && aligned(a.z, 16) && aligned(a.res, 16) && aligned(a.bias, 16) &&
+         a.ldc % n == 0 && a.c_group % n == 0 && (!a.z || a.ldz % n == 0) &&
+         (!a.res || a.ldr % n == 0) && (!a.bias || a.bias_group % n == 0);
 }
 
 enum class Size { Large, Middle, Small };
@@ -724,43 +844,72 @@ struct Choice {
   int splits;
 };
 
-// Tiles of (256, 256), (128, 128) or (64, 64), the largest that leaves a
-// workgroup for most of the 256 compute units; and where the smallest tiles do
-// not, k in parts.
+// What a workgroup of a kind costs, in microseconds as measured: `first` for its
+// launch, first loads and stores; a step of 64 (16 bit) or 32 (f32) k alone on a
+// compute unit and with the `fit` of them that one holds.
+struct Kind {
+  Size size;
+  int bm, bn, fit;
+  double first, alone, full;
+};
+
+const Kind kDirect[] = {{Size::Large, 256, 256, 1, 12.0, 1.95, 1.95},
+                        {Size::Middle, 128, 128, 2, 6.0, 0.75, 1.2},
+                        {Size::Small, 64, 64, 5, 4.0, 0.45, 1.1}};
+const Kind kThrough[] = {{Size::Middle, 128, 128, 2, 6.0, 1.2, 1.6},
+                         {Size::Small, 64, 64, 4, 4.0, 1.1, 1.4}};
+const Kind kF32[] = {{Size::Middle, 128, 128, 2, 9.0, 1.95, 2.7},
+                     {Size::Small, 64, 128, 3, 6.0, 1.45, 2.3}};
+
+// The tile and the parts of k whose estimate is the least: large tiles read each
+// operand less often, small ones and parts of k fill the 256 compute units.
 Choice choose(const Args& a) {
-  const bool weight = a.form == FEDTRAIN_GRAD_WEIGHT;
-  const int64_t groups = a.groups ? a.groups : 1;
-  auto tiles = [&](int64_t b) {
-    const int64_t n = a.n ? (a.n + b - 1) / b : 1;
-    const int64_t m = weight ? (a.m + b - 1) / b * groups
-                             : (a.m + b - 1) / b + (a.groups ? a.groups / 2 : 0);
-    return m * n;
-  };
-  const int64_t rows = weight ? a.m : a.m / groups;  // of one weight matrix
-  if (a.dtype != FEDTRAIN_F32 && in_eights(a) && rows >= 192 && a.n >= 192 && tiles(256) >= 192)
-    return {Size::Large, 1};
-  if (rows >= 96 && a.n >= 96 && tiles(128) >= 192) return {Size::Middle, 1};
-  int64_t splits = 1;
-  const int64_t have = tiles(64), steps = (a.k + 63) / 64;
-  if (!(weight && a.groups) && have > 0 && have < 256) {
-    splits = (512 + have - 1) / have;
-    if (splits > steps / 4) splits = steps / 4;
-    if (splits > 64) splits = 64;
-    if (splits < 1) splits = 1;
+  const bool weight = a.form == FEDTRAIN_GRAD_WEIGHT, f32 = a.dtype == FEDTRAIN_F32;
+  const bool d = in_eights(a);
+  const Kind* kinds = f32 ? kF32 : d ? kDirect : kThrough;
+  const int count = !f32 && d ? 3 : 2;
+  const double groups = a.groups ? a.groups : 1;
+  const double k = weight ? a.k / groups : a.k, bk = f32 ? 32 : 64;
+  const double steps = std::ceil(k / bk) + (weight && a.groups ? 0.5 : 0.0);
+  Choice best = {Size::Small, 1};
+  double least = 1e30;
+  for (int i = 0; i < count; ++i) {
+    const Kind& t = kinds[i];
+    if (t.size == Size::Large && weight) continue;  // its registers do not suffice
+    double tiles = std::ceil(a.n / static_cast<double>(t.bn));
+    if (tiles < 1) tiles = 1;
+    if (weight) tiles *= std::ceil(a.m / static_cast<double>(t.bm)) * groups;
+    else if (!a.groups) tiles *= std::ceil(a.m / static_cast<double>(t.bm));
+    else tiles *= groups * std::max(1.0, a.m / groups / t.bm + 0.5);  // ragged
+    for (int s = 1; s <= 32; s += s < 4 ? 1 : s < 8 ? 2 : s / 2) {
+      if (s > 1 && (steps < 2 * s || (weight && a.groups) || t.size == Size::Large)) break;
+      const double each = tiles * s / 256;  // workgroups a compute unit
+      const double held = each < t.fit ? std::max(1.0, std::ceil(each)) : t.fit;
+      const double step =
+          t.fit > 1 ? t.alone + (t.full - t.alone) * (held - 1) / (t.fit - 1) : t.full;
+      const double rounds = each < t.fit ? 1.0 : each < 4 * t.fit ? std::ceil(each / t.fit)
+                                                                  : each / t.fit + 0.5;
+      double cost = rounds * (t.first + std::ceil(steps / s) * step);
+      if (s > 1) cost += 4.0 + s * static_cast<double>(a.m) * a.n * 8 / 3e6;  // k_join
+      if (cost < least) {
+        least = cost;
+        best = {t.size, s};
+      }
+    }
   }
-  return {Size::Small, static_cast<int>(splits)};
+  return best;
 }
 
 int64_t workspace(const Args& a) {
   const int s = choose(a).splits;
   if (s < 2) return 0;
-  return static_cast<int64_t>(s) * a.m * ((a.n + 3) / 4 * 4 + (a.colsum ? 4 : 0)) * 4;
+  return static_cast<int64_t>(s) * a.m * ((a.n + 7) / 8 * 8 + (a.colsum ? 8 : 0)) * 4;
 }
 
-template <int D, int FORM, class S, bool DIRECT> int go(const Args& a, int splits, hipStream_t s) {
+template <int D, int FORM, class S> int go(const Args& a, int splits, hipStream_t s) {
   Plan p;
   p.splits = splits;
-  p.wide = in_fours(a);
+  p.wide = out_in_eights(a);
   p.tiles_n = a.n ? (a.n + S::BN - 1) / S::BN : 1;
   int64_t all;
   if (FORM == FEDTRAIN_GRAD_WEIGHT) {
@@ -770,10 +919,19 @@ template <int D, int FORM, class S, bool DIRECT> int go(const Args& a, int split
     all = p.tiles_m = a.groups ? a.m / S::BM + a.groups + 2 : (a.m + S::BM - 1) / S::BM;
   }
   if (all > INT32_MAX / p.tiles_n) return FEDTRAIN_EINVAL;
+  // Bands of 4 (forward), 2 (grad input) and 8 rows (grad weight) took 1026, 1060
+  // and 1122 us where 8, 8 and 4 took 1035, 1159 and 1151 (8192 x 4096 x 16384
+  // bf16).  Ragged groups have weights of their own: the columns of one row of
+  // tiles at a time read them in whole rows (64 experts 600 and 714 us, against
+  // 695 and 1013 in bands of 8).
+  p.high = FORM == FEDTRAIN_FORWARD ? 4 : FORM == FEDTRAIN_GRAD_INPUT ? 2 : 8;
+  if (a.groups) p.high = FORM == FEDTRAIN_GRAD_WEIGHT ? 16 : 1;
   constexpr int PLANES = D == FEDTRAIN_F32 ? 3 : 1;
-  constexpr int BYTES = (DIRECT ? 2 : 1) * PLANES * (S::BM + S::BN) * S::BK * 2 +
-                        (D == FEDTRAIN_F32 ? 16 : 0);  // and the mark of an infinity
-  auto* kernel = &k_product<D, FORM, S, DIRECT>;
+  constexpr int STAGES = S::STAGES * PLANES * (S::BM + S::BN) * S::BK * 2;
+  // and the mark of an infinity
+  constexpr int BYTES = STAGES + (D == FEDTRAIN_F32 ? 16 : 0);
+  static_assert(S::PASS * 16 * S::BN * S::MW * 4 <= STAGES, "what leaves through LDS fits it");
+  auto* kernel = &k_product<D, FORM, S>;
   if (BYTES > 64 * 1024) {
     // for the current device; it costs about a microsecond
     const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
@@ -784,9 +942,9 @@ template <int D, int FORM, class S, bool DIRECT> int go(const Args& a, int split
                      dim3(S::THREADS), BYTES, s, a, p);
   if (splits > 1) {
     if (const int rc = launched()) return rc;
-    const int64_t fours = a.m * ((a.n + 3) / 4 + (a.colsum ? 1 : 0));
-    if (fours > static_cast<int64_t>(INT32_MAX) * 256) return FEDTRAIN_EINVAL;
-    hipLaunchKernelGGL((k_join<D, FORM>), dim3(static_cast<unsigned>((fours + 255) / 256)),
+    const int64_t eights = a.m * ((a.n + 7) / 8 + (a.colsum ? 1 : 0));
+    if (eights > static_cast<int64_t>(INT32_MAX) * 256) return FEDTRAIN_EINVAL;
+    hipLaunchKernelGGL((k_join<D, FORM>), dim3(static_cast<unsigned>((eights + 255) / 256)),
                        dim3(256), 0, s, a, p);
   }
   return launched();
@@ -798,16 +956,17 @@ template <int D, int FORM> int run(const Args& a, hipStream_t s) {
                        a.workspace_bytes < workspace(a)))
     return FEDTRAIN_EINVAL;
   if constexpr (D == FEDTRAIN_F32) {
-    if (c.size == Size::Small) return go<D, FORM, Shape<2, 2, 2, 2, 32>, false>(a, c.splits, s);
-    return go<D, FORM, Shape<2, 2, 4, 4, 32>, false>(a, 1, s);
+    if (c.size == Size::Small) return go<D, FORM, Shape<1, 4, 4, 2, 32, 2>>(a, c.splits, s);
+    return go<D, FORM, Shape<2, 2, 4, 4, 32, 2>>(a, c.splits, s);
   } else {
-    if (c.size == Size::Large) return go<D, FORM, Shape<2, 4, 8, 4, 64>, true>(a, 1, s);
+    if constexpr (FORM != FEDTRAIN_GRAD_WEIGHT)
+      if (c.size == Size::Large) return go<D, FORM, Shape<2, 4, 8, 4, 64, 4, 2>>(a, 1, s);
     const bool d = in_eights(a);
-    if (c.size == Size::Middle)
-      return d ? go<D, FORM, Shape<2, 2, 4, 4, 64>, true>(a, 1, s)
-               : go<D, FORM, Shape<2, 2, 4, 4, 64>, false>(a, 1, s);
-    return d ? go<D, FORM, Shape<2, 2, 2, 2, 64>, true>(a, c.splits, s)
-             : go<D, FORM, Shape<2, 2, 2, 2, 64>, false>(a, c.splits, s);
+    if (c.size != Size::Small)
+      return d ? go<D, FORM, Shape<2, 2, 4, 4, 64, 4, 2>>(a, c.splits, s)
+               : go<D, FORM, Shape<2, 2, 4, 4, 64, 2>>(a, c.splits, s);
+    return d ? go<D, FORM, Shape<2, 2, 2, 2, 64, 2, 2>>(a, c.splits, s)
+             : go<D, FORM, Shape<2, 2, 2, 2, 64, 2>>(a, c.splits, s);
   }
 }
 
