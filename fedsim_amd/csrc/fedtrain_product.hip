@@ -246,24 +246,46 @@ template <int D, class L, int THREADS, bool DIRECT> struct Loader {
 
   // DIRECT: memory to LDS without registers.  A lane outside the operand asks
   // for an offset past the descriptor's range, which stores zeros.
-  __device__ void issue(int64_t k, int64_t k1, char* to, int tid) const {
-    if (k > k1) k = k1;  // past the end every lane asks for zeros
-    const int64_t first = L::KS ? k * ld : k;
-    auto d = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base + first), 0, 0x7FFFFFFF,
-                                               0x00027000);
-    const int left = k1 - k < L::BK ? static_cast<int>(k1 - k) : L::BK;
-    to += __builtin_amdgcn_readfirstlane(tid & ~63) * 16;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      unsigned o = offset[i];
-      if (left < L::BK) {
-        const int q = tid + i * THREADS, line = q / L::per_line;
-        const int c = (q % L::per_line) ^ L::swizzle(line);
-        if (L::KS ? line >= left : c * 8 >= left) o = ~0u;
-      }
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          d, (__attribute__((address_space(3))) void*)(to + i * THREADS * 16), 16, o, 0, 0, 0);
+  //
+  // The loads are written out because the compiler, which cannot tell the stages
+  // apart, would wait for all of them before the next LDS read: arrive() and
+  // wait_loads() are what orders them.  They have no result in a register.  Five
+  // cycles go by before a load reads scalar registers, in case the vector unit
+  // wrote them.
+  __device__ u32x4 descriptor(int64_t k) const {
+    const uint64_t p = reinterpret_cast<uint64_t>(base + (L::KS ? k * ld : k));
+    u32x4 d;
+    d[0] = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(p));
+    d[1] = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(p >> 32) & 0xFFFFu);
+    d[2] = 0x7FFFFFFFu;
+    d[3] = 0x00027000u;
+    return d;
+  }
+  // load i of a stage, of which `left` k exist (FULL: all)
+  template <bool FULL>
+  __device__ void issue(int i, u32x4 d, int left, const char* to, int tid) const {
+    unsigned o = offset[i];
+    if (!FULL) {
+      const int q = tid + i * THREADS, line = q / L::per_line;
+      const int c = (q % L::per_line) ^ L::swizzle(line);
+      if (L::KS ? line >= left : c * 8 >= left) o = ~0u;
     }
+    const unsigned at = __builtin_amdgcn_readfirstlane(
+        static_cast<unsigned>(reinterpret_cast<uintptr_t>(
+            (const __attribute__((address_space(3))) char*)to)) +
+        ((tid & ~63) + i * THREADS) * 16);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"(at), "v"(o), "s"(d)
+                 : "memory");
+  }
+  // the stage at k, of which some, all or no k exist
+  __device__ void issue_all(int64_t k, int64_t k1, char* to, int tid) const {
+    if (k > k1) k = k1;
+    const u32x4 d = descriptor(k);
+    const int left = k1 - k < L::BK ? static_cast<int>(k1 - k) : L::BK;
+#pragma unroll
+    for (int i = 0; i < N; ++i) issue<false>(i, d, left, to, tid);
   }
 
   // through registers: any alignment, any length.  For steps of BK from k on.
@@ -341,6 +363,7 @@ template <int D, class L, int THREADS, bool DIRECT> struct Loader {
 // PASS of the MI at a time are written to C.  STAGES of tiles in LDS: 1 where they
 // come through registers, more where they come without.
 template <int MW_, int NW_, int MI_, int NI_, int BK_, int PASS_, int STAGES_ = 1> struct Shape {
+  static constexpr int WAVES = MI_ * NI_ > 32 ? 1 : 2;  // of a SIMD: what registers allow
   static constexpr bool DIRECT = STAGES_ > 1;
   static constexpr int STAGES = STAGES_;
   static constexpr int MW = MW_, NW = NW_, MI = MI_, NI = NI_, BK = BK_, PASS = PASS_;
@@ -442,7 +465,7 @@ __device__ inline void put(const Args& a, int group, int64_t row, int64_t col, i
   const int64_t first = FORM == FEDTRAIN_GRAD_WEIGHT ? group * a.c_group : 0;
   write8<D>(a.c, first + row * a.ldc + col, n, wide, v);
 }
-template <int D, int FORM, class S> __global__ __launch_bounds__(S::THREADS, 2)
+template <int D, int FORM, class S> __global__ __launch_bounds__(S::THREADS, S::WAVES)
 void k_product(Args a, Plan plan) {
 #ifdef __HIP_DEVICE_COMPILE__  // the host's pass needs the name alone
   using T = typename Elem<D>::type;
@@ -453,7 +476,8 @@ void k_product(Args a, Plan plan) {
   constexpr int STAGE = PLANES * (LA::bytes + LB::bytes);
   extern __shared__ __attribute__((aligned(1024))) char lds[];
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / S::NW * (S::MI * 16), wn = wave % S::NW * (S::NI * 16);
   int64_t slot, tn;
   place(plan.tiles_m * (WEIGHT && a.groups ? a.groups : 1), plan.tiles_n, plan.high, slot, tn);
@@ -518,30 +542,48 @@ void k_product(Args a, Plan plan) {
 #pragma unroll
       for (int i = 0; i < S::MI; ++i) f.a[i] = LA::fragment(at, wm, i, kk, lane);
     };
-    // a step's products, and between them the next step's reads
+    constexpr int LOADS = LA::chunks / S::THREADS + LB::chunks / S::THREADS;
+    auto issue = [&](int64_t k, char* to) {
+      la.issue_all(k, k1, to, tid);
+      lb.issue_all(k, k1, to + LA::bytes, tid);
+    };
+    // A step's products; between them the next step's reads, and the loads of the
+    // stage at k where `loads`, in the order written (the unit takes a product
+    // every 16 cycles; a read or a load in between costs it nothing, a row of them
+    // does).
     auto multiply = [&](const Fragments& f, Fragments& other, const char* at, int kk,
-                        auto with_sum) {
-      if (!live) return;
-      read(other, at, kk);
-#pragma unroll
-      for (int i = 0; i < S::MI; ++i) {
-#pragma unroll
-        for (int j = 0; j < S::NI; ++j) acc[i][j] = mfma<D>(f.b[j], f.a[i], acc[i][j]);
-        if constexpr (decltype(with_sum)::value) sum[i] = mfma<D>(one, f.a[i], sum[i]);
+                        auto with_sum, auto loads, int64_t k, char* to) {
+      constexpr bool LOAD = decltype(loads)::value;
+      constexpr int NA = decltype(la)::N, NB = decltype(lb)::N;
+      const auto da = la.descriptor(LOAD ? k : k0), db = lb.descriptor(LOAD ? k : k0);
+      if (!live) {
+        if (LOAD) issue(k, to);
+        return;
       }
-      constexpr int READS = S::NI * (LB::KS ? 2 : 1) + S::MI * (LA::KS ? 2 : 1);
-      constexpr int EACH = S::MI * S::NI / READS > 0 ? S::MI * S::NI / READS : 1;
+      constexpr int READS = S::NI + S::MI;
+      constexpr int ALL = S::MI * S::NI, EACH = (ALL + READS - 1) / READS;
+      constexpr int LOADS_EACH = (NA + NB + READS - 1) / READS;
 #pragma unroll
       for (int r = 0; r < READS; ++r) {
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);   // an LDS read
-        __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);  // products
+        if (r < S::NI) other.b[r < S::NI ? r : 0] = LB::fragment(at + LA::bytes, wn, r, kk, lane);
+        else other.a[r < S::NI ? 0 : r - S::NI] = LA::fragment(at, wm, r - S::NI, kk, lane);
+        if (LOAD) {
+#pragma unroll
+          for (int l = r * LOADS_EACH; l < (r + 1) * LOADS_EACH && l < NA + NB; ++l) {
+            if (l < NA) la.template issue<true>(l < NA ? l : 0, da, 0, to, tid);
+            else lb.template issue<true>(l < NA ? 0 : l - NA, db, 0, to + LA::bytes, tid);
+          }
+        }
+#pragma unroll
+        for (int t = r * EACH; t < (r + 1) * EACH && t < ALL; ++t) {
+          const int i = t / S::NI, j = t % S::NI;
+          acc[i][j] = mfma<D>(f.b[j], f.a[i], acc[i][j]);
+          if constexpr (decltype(with_sum)::value)
+            if (j == 0) sum[i] = mfma<D>(one, f.a[i], sum[i]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     };
-    auto issue = [&](int64_t k, char* to) {
-      la.issue(k, k1, to, tid);
-      lb.issue(k, k1, to + LA::bytes, tid);
-    };
-    constexpr int LOADS = LA::chunks / S::THREADS + LB::chunks / S::THREADS;
     auto loop = [&](auto with_sum) {
       Fragments f[2];
       issue(k0, lds);
@@ -550,14 +592,19 @@ void k_product(Args a, Plan plan) {
       arrive();
       if (live) read(f[0], lds, 0);
       int turn = 0;
-      for (int64_t k = k0; k < k1; k += S::BK, turn ^= 1) {
+      auto stage = [&](int64_t k, auto loads) {
         char* now = lds + turn * STAGE;
-        multiply(f[0], f[1], now, 1, with_sum);
+        turn ^= 1;
+        multiply(f[0], f[1], now, 1, with_sum, std::false_type(), 0, nullptr);
         wait_loads<0>();
         arrive();
-        if (k + 2 * S::BK < k1) issue(k + 2 * S::BK, now);
-        multiply(f[1], f[0], lds + (turn ^ 1) * STAGE, 0, with_sum);
-      }
+        if (!decltype(loads)::value && k + 2 * S::BK < k1)
+          issue(k + 2 * S::BK, now);
+        multiply(f[1], f[0], lds + turn * STAGE, 0, with_sum, loads, k + 2 * S::BK, now);
+      };
+      int64_t k = k0;
+      for (; k + 3 * S::BK <= k1; k += S::BK) stage(k, std::true_type());
+      for (; k < k1; k += S::BK) stage(k, std::false_type());
     };
     if (k0 < k1) {
       if constexpr (WEIGHT) {
@@ -960,7 +1007,7 @@ template <int D, int FORM> int run(const Args& a, hipStream_t s) {
     return go<D, FORM, Shape<2, 2, 4, 4, 32, 2>>(a, c.splits, s);
   } else {
     if constexpr (FORM != FEDTRAIN_GRAD_WEIGHT)
-      if (c.size == Size::Large) return go<D, FORM, Shape<2, 4, 8, 4, 64, 4, 2>>(a, 1, s);
+      if (c.size == Size::Large) return go<D, FORM, Shape<2, 2, 8, 8, 64, 4, 2>>(a, 1, s);
     const bool d = in_eights(a);
     if (c.size != Size::Small)
       return d ? go<D, FORM, Shape<2, 2, 4, 4, 64, 4, 2>>(a, c.splits, s)
