@@ -249,9 +249,9 @@ template <int D, class L, int THREADS, bool DIRECT> struct Loader {
   //
   // The loads are written out because the compiler, which cannot tell the stages
   // apart, would wait for all of them before the next LDS read: arrive() and
-  // wait_loads() are what orders them.  They have no result in a register.  Five
-  // cycles go by before a load reads scalar registers, in case the vector unit
-  // wrote them.
+  // wait_loads() are what orders them.  They have no result in a register.  A
+  // descriptor's registers may come from the vector unit, 5 cycles before a load
+  // may read them.
   __device__ u32x4 descriptor(int64_t k) const {
     const uint64_t p = reinterpret_cast<uint64_t>(base + (L::KS ? k * ld : k));
     u32x4 d;
@@ -259,6 +259,7 @@ template <int D, class L, int THREADS, bool DIRECT> struct Loader {
     d[1] = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(p >> 32) & 0xFFFFu);
     d[2] = 0x7FFFFFFFu;
     d[3] = 0x00027000u;
+    asm volatile("s_nop 4" : "+s"(d));
     return d;
   }
   // load i of a stage, of which `left` k exist (FULL: all)
@@ -274,7 +275,7 @@ template <int D, class L, int THREADS, bool DIRECT> struct Loader {
         static_cast<unsigned>(reinterpret_cast<uintptr_t>(
             (const __attribute__((address_space(3))) char*)to)) +
         ((tid & ~63) + i * THREADS) * 16);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :
                  : "s"(at), "v"(o), "s"(d)
                  : "memory");
@@ -437,34 +438,59 @@ template <int D> __device__ inline void write8(void* p, int64_t at, int n, bool 
   }
 }
 
-// n neighbouring sums of a row of C (8, where wide), to their end
-template <int D, int FORM, int ACT>
-__device__ inline void put(const Args& a, int group, int64_t row, int64_t col, int n, bool wide,
-                           float* v) {
-  if constexpr (FORM == FEDTRAIN_FORWARD) {
-    if (group >= 0) {
-      if (a.bias) {
-        float b[8];
-        read8<D>(a.bias, group * a.bias_group + col, n, wide, b);
+// Where eight neighbouring columns of C are written, row by row.
+template <int D, int FORM> struct Out {
+  using T = typename Elem<D>::type;
+  T *c, *z;
+  const T* res;
+  float bias[8];
+  int n;
+  bool wide, held;  // held: by a group; other rows get their residual
+
+  __device__ Out(const Args& a, bool wide_, int group, int64_t row, int64_t col, int64_t n_)
+      : n(static_cast<int>(n_ < 8 ? n_ : 8)), wide(wide_ && n_ >= 8), held(group >= 0) {
+    const int64_t first = FORM == FEDTRAIN_GRAD_WEIGHT ? group * a.c_group : 0;
+    c = static_cast<T*>(a.c) + first + row * a.ldc + col;
+    if constexpr (FORM == FEDTRAIN_FORWARD) {
+      z = a.z ? static_cast<T*>(a.z) + row * a.ldz + col : nullptr;
+      res = a.res ? static_cast<const T*>(a.res) + row * a.ldr + col : nullptr;
+      if (a.bias && held && n > 0) {
+        read8<D>(a.bias, group * a.bias_group + col, n, wide, bias);
+      } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += b[e];
+        for (int e = 0; e < 8; ++e) bias[e] = 0;
       }
-      if (a.z) write8<D>(a.z, row * a.ldz + col, n, wide, v);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = act_value<D, ACT>(v[e]);
-    } else if (a.z) {
-      write8<D>(a.z, row * a.ldz + col, n, wide, v);
-    }
-    if (a.res) {
-      float r[8];
-      read8<D>(a.res, row * a.ldr + col, n, wide, r);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] += r[e];
     }
   }
-  const int64_t first = FORM == FEDTRAIN_GRAD_WEIGHT ? group * a.c_group : 0;
-  write8<D>(a.c, first + row * a.ldc + col, n, wide, v);
-}
+  // to the row `rows` further down
+  __device__ void advance(const Args& a, int rows) {
+    c += rows * a.ldc;
+    if constexpr (FORM == FEDTRAIN_FORWARD) {
+      if (z) z += rows * a.ldz;
+      if (res) res += rows * a.ldr;
+    }
+  }
+  // a row's sums, to their end
+  template <int ACT> __device__ void put(float* v) const {
+    if constexpr (FORM == FEDTRAIN_FORWARD) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += bias[e];
+      if (z) write8<D>(z, 0, n, wide, v);
+      if (held) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = act_value<D, ACT>(v[e]);
+      }
+      if (res) {
+        float r[8];
+        read8<D>(res, 0, n, wide, r);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += r[e];
+      }
+    }
+    write8<D>(c, 0, n, wide, v);
+  }
+};
+
 template <int D, int FORM, class S> __global__ __launch_bounds__(S::THREADS, S::WAVES)
 void k_product(Args a, Plan plan) {
 #ifdef __HIP_DEVICE_COMPILE__  // the host's pass needs the name alone
@@ -555,10 +581,14 @@ void k_product(Args a, Plan plan) {
                         auto with_sum, auto loads, int64_t k, char* to) {
       constexpr bool LOAD = decltype(loads)::value;
       constexpr int NA = decltype(la)::N, NB = decltype(lb)::N;
-      const auto da = la.descriptor(LOAD ? k : k0), db = lb.descriptor(LOAD ? k : k0);
+      u32x4 da, db;
       if (!live) {
         if (LOAD) issue(k, to);
         return;
+      }
+      if constexpr (LOAD) {
+        da = la.descriptor(k);
+        db = lb.descriptor(k);
       }
       constexpr int READS = S::NI + S::MI;
       constexpr int ALL = S::MI * S::NI, EACH = (ALL + READS - 1) / READS;
@@ -598,8 +628,7 @@ void k_product(Args a, Plan plan) {
         multiply(f[0], f[1], now, 1, with_sum, std::false_type(), 0, nullptr);
         wait_loads<0>();
         arrive();
-        if (!decltype(loads)::value && k + 2 * S::BK < k1)
-          issue(k + 2 * S::BK, now);
+        if (!decltype(loads)::value && k + 2 * S::BK < k1) issue(k + 2 * S::BK, now);
         multiply(f[1], f[0], lds + turn * STAGE, 0, with_sum, loads, k + 2 * S::BK, now);
       };
       int64_t k = k0;
@@ -739,9 +768,12 @@ void k_product(Args a, Plan plan) {
   // The sums go through the wave's own part of LDS, some rows at a time, and come
   // back as eight neighbours of a row, rows one after another: whole lines of
   // memory, and one copy of the code that follows.
-  constexpr int LINE = S::NI * 16, EIGHTS = S::NI * 2, FIT = S::PASS;
+  constexpr int LINE = S::NI * 16, EIGHTS = S::NI * 2, FIT = S::PASS, DOWN = 64 / EIGHTS;
   f32x4* mine = reinterpret_cast<f32x4*>(lds) + wave * (FIT * 16 * LINE / 4);
   auto spot = [](int row, int four) { return row * (LINE / 4) + (four ^ (row & (LINE / 4 - 1))); };
+  const int c8 = lane % EIGHTS, c = wn + c8 * 8, n = static_cast<int>(cols) - c;
+  int r = wm + lane / EIGHTS;
+  Out<D, FORM> out(a, plan.wide, group, row0 + r, col0 + c, n);
 #pragma unroll
   for (int i0 = 0; i0 < S::MI; i0 += FIT) {
 #pragma unroll
@@ -750,22 +782,21 @@ void k_product(Args a, Plan plan) {
       for (int j = 0; j < S::NI; ++j)
         mine[spot(i * 16 + (lane & 15), j * 4 + (lane >> 4))] = acc[i0 + i][j];
     by_act(FORM == FEDTRAIN_FORWARD ? a.act : 0, [&](auto act) {
-#pragma unroll 2
-      for (int u = lane; u < FIT * 16 * EIGHTS; u += 64) {
-        const int row = u / EIGHTS, c8 = u % EIGHTS;
+#pragma unroll 4
+      for (int row = lane / EIGHTS; row < FIT * 16; row += DOWN, r += DOWN) {
         const f32x4 lo = mine[spot(row, c8 * 2)], hi = mine[spot(row, c8 * 2 + 1)];
         float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        const int r = wm + i0 * 16 + row, c = wn + c8 * 8, n = static_cast<int>(cols) - c;
-        if (r >= rows || n <= 0) continue;
-        if (plan.splits > 1) {
-          Eight<float> f;
+        if (r < rows && n > 0) {
+          if (plan.splits > 1) {
+            Eight<float> f;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f.v[e] = v[e];
-          *reinterpret_cast<Eight<float>*>(partial + r * width + col0 + c) = f;
-        } else {
-          put<D, FORM, decltype(act)::value>(a, group, row0 + r, col0 + c, n,
-                                             plan.wide && n >= 8, v);
+            for (int e = 0; e < 8; ++e) f.v[e] = v[e];
+            *reinterpret_cast<Eight<float>*>(partial + r * width + col0 + c) = f;
+          } else {
+            out.template put<decltype(act)::value>(v);
+          }
         }
+        out.advance(a, DOWN);
       }
     });
   }
@@ -798,10 +829,9 @@ template <int D, int FORM> __global__ __launch_bounds__(256) void k_join(Args a,
     if (group < 0)
       for (int e = 0; e < 8; ++e) v[e] = 0;
   }
-  const int n = static_cast<int>(a.n - col < 8 ? a.n - col : 8);
-  by_act(FORM == FEDTRAIN_FORWARD ? a.act : 0, [&](auto act) {
-    put<D, FORM, decltype(act)::value>(a, group, row, col, n, plan.wide && n >= 8, v);
-  });
+  const Out<D, FORM> out(a, plan.wide, group, row, col, a.n - col);
+  by_act(FORM == FEDTRAIN_FORWARD ? a.act : 0,
+         [&](auto act) { out.template put<decltype(act)::value>(v); });
 }
 
 // dz = dy act'(z): one pass, eight values a thread where rows allow it
@@ -900,7 +930,7 @@ struct Kind {
   double first, alone, full;
 };
 
-const Kind kDirect[] = {{Size::Large, 256, 256, 1, 12.0, 1.95, 1.95},
+const Kind kDirect[] = {{Size::Large, 256, 256, 1, 12.0, 1.7, 1.7},
                         {Size::Middle, 128, 128, 2, 6.0, 0.75, 1.2},
                         {Size::Small, 64, 64, 5, 4.0, 0.45, 1.1}};
 const Kind kThrough[] = {{Size::Middle, 128, 128, 2, 6.0, 1.2, 1.6},
@@ -922,7 +952,6 @@ Choice choose(const Args& a) {
   double least = 1e30;
   for (int i = 0; i < count; ++i) {
     const Kind& t = kinds[i];
-    if (t.size == Size::Large && weight) continue;  // its registers do not suffice
     double tiles = std::ceil(a.n / static_cast<double>(t.bn));
     if (tiles < 1) tiles = 1;
     if (weight) tiles *= std::ceil(a.m / static_cast<double>(t.bm)) * groups;
@@ -1006,8 +1035,7 @@ template <int D, int FORM> int run(const Args& a, hipStream_t s) {
     if (c.size == Size::Small) return go<D, FORM, Shape<1, 4, 4, 2, 32, 2>>(a, c.splits, s);
     return go<D, FORM, Shape<2, 2, 4, 4, 32, 2>>(a, c.splits, s);
   } else {
-    if constexpr (FORM != FEDTRAIN_GRAD_WEIGHT)
-      if (c.size == Size::Large) return go<D, FORM, Shape<2, 2, 8, 8, 64, 4, 2>>(a, 1, s);
+    if (c.size == Size::Large) return go<D, FORM, Shape<2, 2, 8, 8, 64, 4, 2>>(a, 1, s);
     const bool d = in_eights(a);
     if (c.size != Size::Small)
       return d ? go<D, FORM, Shape<2, 2, 4, 4, 64, 4, 2>>(a, c.splits, s)
