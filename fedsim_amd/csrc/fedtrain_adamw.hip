@@ -24,12 +24,19 @@ namespace {
 using namespace fedtrain;
 
 constexpr int kBlock = 256;   // elements that share a scale: 64 lanes x 4
-constexpr int kMost = 40;     // tensors a launch takes: 40 x 72 B of kernel arguments
+constexpr int kMost = 62;     // tensors a launch takes: 62 x 64 B of the 4 KiB of arguments
 
 struct Tensor {
-  fedtrain_adamw_tensor t;
-  int first;  // the tensor's first workgroup
-  int wide;   // every pointer allows loads of 4 elements
+  void* p;
+  const void* g;
+  void *m, *v;
+  float *m_scale, *v_scale;
+  int64_t n_wide;  // 2 n, + 1 where every pointer is 16-byte aligned
+  int first;       // the tensor's first workgroup
+  unsigned block0;
+
+  __device__ int64_t n() const { return n_wide >> 1; }
+  __device__ bool wide() const { return n_wide & 1; }
 };
 
 struct Batch {
@@ -37,7 +44,6 @@ struct Batch {
   int count;
   float b1, c1, b2, c2, decay, eps, size, root;
   unsigned key;
-  float sign;
   const float* device;  // {size, root, key} computed on the device, or null
 };
 
@@ -61,22 +67,13 @@ template <int TOP> __device__ inline int scale_exponent(float most) {
   return e < 1 ? 1 : e;
 }
 
-// |x| in units of the scale, rounded to a float of MANT bits and smallest
-// normal 2^LEAST: up with the probability of the part that is cut off
-template <int MANT, int LEAST> __device__ inline float stochastic(float a, unsigned u16) {
-  unsigned e = to_bits(a) >> 23;
-  e = e < 127 + LEAST ? 127 + LEAST : e;
-  float up = from_bits((254 - e + MANT) << 23), step = from_bits((e - MANT) << 23);
-  return floorf(a * up + static_cast<float>(u16) * 0x1p-16f) * step;
-}
-
 struct Moments {
   float m, v;
 };
 
-__device__ inline Moments moments(const Batch& b, float m, float v, float g) {
-  g *= b.sign;
-  return {m * b.b1 + g * b.c1, v * b.b2 + (g * b.c2) * g};
+// From states that already carry b1 and b2.  c1 has the sign of the direction.
+__device__ inline Moments moments(const Batch& b, float b1m, float b2v, float g) {
+  return {b1m + g * b.c1, b2v + (g * b.c2) * g};
 }
 
 struct Scalars {
@@ -88,7 +85,7 @@ __device__ inline float step_of(const Batch& b, const Scalars& c, float p, Momen
   // the square root and the quotient of the hardware, each within one unit of
   // its last place: far below the rounding of p
   float d = __builtin_amdgcn_sqrtf(s.v) * c.root + b.eps;
-  return p * b.decay - c.size * (s.m * __builtin_amdgcn_rcpf(d));
+  return __builtin_fmaf(p, b.decay, -(c.size * (s.m * __builtin_amdgcn_rcpf(d))));
 }
 
 template <class T, int V> struct __attribute__((aligned(V * sizeof(T)))) Vec {
@@ -111,39 +108,69 @@ template <int SPAN> __device__ inline float span_max(float x) {
 
 // The codes of V neighbouring elements of block `blk`, from its element `first`
 // on; SPAN lanes share the block, and one of them stores its scales.
+//
+// A code is its value rounded down on the grid of codes, or up with the
+// probability of the part that is cut off, floor(x / spacing + u) spacing with u
+// 16 random bits over 2^16: the conversion's own rounding with u in the high half
+// of its random operand, subnormal codes included (compared on 33 million values).
+// An infinity or NaN gets a code of its own: NaN (m), infinity or NaN (v).
 template <int V, int SPAN>
 __device__ inline void requantize(const float* m, const float* v, unsigned key, int64_t blk,
-                                  unsigned first, float* m_scale, float* v_scale,
-                                  unsigned* qm, unsigned* qv) {
-  float mm = 0, vm = 0;
+                                  unsigned first, float* m_scale, float* v_scale, unsigned* qm,
+                                  unsigned* qv) {
+  float mm = 0, vm = 0;  // the maximum of a number and NaN is the number
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    // an infinity or NaN is that element's alone: it does not set the scale
-    mm = fmaxf(mm, fabsf(m[e]) < INFINITY ? fabsf(m[e]) : 0.0f);
-    vm = fmaxf(vm, v[e] < INFINITY ? v[e] : 0.0f);
+    mm = fmaxf(mm, fabsf(m[e]));
+    vm = fmaxf(vm, v[e]);
   }
-  const int me = scale_exponent<7>(span_max<SPAN>(mm));
-  const int ve = scale_exponent<14>(span_max<SPAN>(vm));
+  mm = span_max<SPAN>(mm);
+  vm = span_max<SPAN>(vm);
+  if (__builtin_amdgcn_ballot_w64(!(mm < INFINITY && vm < INFINITY))) {
+    // an infinity does not set its block's scale
+    mm = vm = 0;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      mm = fmaxf(mm, fabsf(m[e]) < INFINITY ? fabsf(m[e]) : 0.0f);
+      vm = fmaxf(vm, v[e] < INFINITY ? v[e] : 0.0f);
+    }
+    mm = span_max<SPAN>(mm);
+    vm = span_max<SPAN>(vm);
+  }
+  const int me = scale_exponent<7>(mm), ve = scale_exponent<14>(vm);
   const float mi = from_bits(static_cast<unsigned>(254 - me) << 23);
   const float vi = from_bits(static_cast<unsigned>(254 - ve) << 23);
   const unsigned bk = mix(key + static_cast<unsigned>(blk) * 0x9E3779B9u);
-  float x[V], y[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    const unsigned h = mix(bk + (first + e) * 0x9E3779B9u);
-    x[e] = copysignf(stochastic<3, -6>(fabsf(m[e]) * mi, h & 0xFFFF), m[e]);
-    y[e] = v[e] * vi;
-    y[e] = y[e] > 0 ? fmaxf(stochastic<2, -14>(y[e], h >> 16), 0x1p-16f) : y[e];
-    // what is no number has a code of its own: NaN (m), infinity or NaN (v)
-    if (!(fabsf(m[e]) < INFINITY)) x[e] = NAN;
-    if (!(v[e] < INFINITY)) y[e] = v[e];
-  }
 #pragma unroll
   for (int e = 0; e < V; e += 4) {
-    int a = __builtin_amdgcn_cvt_pk_fp8_f32(x[e], x[e + 1], 0, false);
-    int c = __builtin_amdgcn_cvt_pk_bf8_f32(y[e], y[e + 1], 0, false);
-    qm[e / 4] = __builtin_amdgcn_cvt_pk_fp8_f32(x[e + 2], x[e + 3], a, true);
-    qv[e / 4] = __builtin_amdgcn_cvt_pk_bf8_f32(y[e + 2], y[e + 3], c, true);
+    int a = 0, c = 0;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const unsigned h = mix(bk + (first + e + s) * 0x9E3779B9u);
+      const float x = m[e + s] * mi;
+      float y = v[e + s] * vi;
+      // v is never rounded to zero, since it divides m: at least the least code
+      if (__builtin_amdgcn_ballot_w64(y < 0x1p-16f)) y = v[e + s] > 0 ? fmaxf(y, 0x1p-16f) : y;
+      switch (s) {  // the byte is a constant of the instruction
+        case 0:
+          a = __builtin_amdgcn_cvt_sr_fp8_f32(x, h << 16, a, 0);
+          c = __builtin_amdgcn_cvt_sr_bf8_f32(y, h & 0xFFFF0000u, c, 0);
+          break;
+        case 1:
+          a = __builtin_amdgcn_cvt_sr_fp8_f32(x, h << 16, a, 1);
+          c = __builtin_amdgcn_cvt_sr_bf8_f32(y, h & 0xFFFF0000u, c, 1);
+          break;
+        case 2:
+          a = __builtin_amdgcn_cvt_sr_fp8_f32(x, h << 16, a, 2);
+          c = __builtin_amdgcn_cvt_sr_bf8_f32(y, h & 0xFFFF0000u, c, 2);
+          break;
+        default:
+          a = __builtin_amdgcn_cvt_sr_fp8_f32(x, h << 16, a, 3);
+          c = __builtin_amdgcn_cvt_sr_bf8_f32(y, h & 0xFFFF0000u, c, 3);
+      }
+    }
+    qm[e / 4] = a;
+    qv[e / 4] = c;
   }
   if ((threadIdx.x & (SPAN - 1)) == 0) {
     *m_scale = from_bits(static_cast<unsigned>(me) << 23);
@@ -155,17 +182,18 @@ __device__ inline void requantize(const float* m, const float* v, unsigned key, 
 template <int D, int BITS, int V>
 __device__ inline void step_wide(const Batch& b, const Scalars& c, const Tensor& t, int64_t at) {
   using T = typename Elem<D>::type;
-  const Vec<T, V> p = get<T, V>(t.t.p, at), g = get<T, V>(t.t.g, at);
+  const Vec<T, V> p = get<T, V>(t.p, at), g = get<T, V>(t.g, at);
   float m[V], v[V];
   const int64_t blk = at / kBlock;
   if constexpr (BITS == 32) {
-    const Vec<float, V> mo = get<float, V>(t.t.m, at), vo = get<float, V>(t.t.v, at);
+    const Vec<float, V> mo = get<float, V>(t.m, at), vo = get<float, V>(t.v, at);
 #pragma unroll
-    for (int e = 0; e < V; ++e) m[e] = mo.v[e], v[e] = vo.v[e];
+    for (int e = 0; e < V; ++e) m[e] = mo.v[e] * b.b1, v[e] = vo.v[e] * b.b2;
   } else {
-    const Vec<unsigned, V / 4> mo = get<unsigned, V / 4>(t.t.m, at / 4);
-    const Vec<unsigned, V / 4> vo = get<unsigned, V / 4>(t.t.v, at / 4);
-    const float ms = t.t.m_scale[blk], vs = t.t.v_scale[blk];
+    const Vec<unsigned, V / 4> mo = get<unsigned, V / 4>(t.m, at / 4);
+    const Vec<unsigned, V / 4> vo = get<unsigned, V / 4>(t.v, at / 4);
+    // a power of two times b1 is exact, and so is code * scale: one rounding
+    const float ms = t.m_scale[blk] * b.b1, vs = t.v_scale[blk] * b.b2;
 #pragma unroll
     for (int e = 0; e < V; e += 4) {
       m[e] = __builtin_amdgcn_cvt_f32_fp8(mo.v[e / 4], 0) * ms;
@@ -186,19 +214,19 @@ __device__ inline void step_wide(const Batch& b, const Scalars& c, const Tensor&
     v[e] = s.v;
     out.v[e] = Elem<D>::down(step_of(b, c, Elem<D>::up(p.v[e]), s));
   }
-  set<T, V>(t.t.p, at, out);
+  set<T, V>(t.p, at, out);
   if constexpr (BITS == 32) {
     Vec<float, V> mo, vo;
 #pragma unroll
     for (int e = 0; e < V; ++e) mo.v[e] = m[e], vo.v[e] = v[e];
-    set<float, V>(t.t.m, at, mo);
-    set<float, V>(t.t.v, at, vo);
+    set<float, V>(t.m, at, mo);
+    set<float, V>(t.v, at, vo);
   } else {
     Vec<unsigned, V / 4> qm, qv;
-    requantize<V, kBlock / V>(m, v, c.key, t.t.block0 + blk, at % kBlock, t.t.m_scale + blk,
-                              t.t.v_scale + blk, qm.v, qv.v);
-    set<unsigned, V / 4>(t.t.m, at / 4, qm);
-    set<unsigned, V / 4>(t.t.v, at / 4, qv);
+    requantize<V, kBlock / V>(m, v, c.key, t.block0 + blk, at % kBlock, t.m_scale + blk,
+                              t.v_scale + blk, qm.v, qv.v);
+    set<unsigned, V / 4>(t.m, at / 4, qm);
+    set<unsigned, V / 4>(t.v, at / 4, qv);
   }
 }
 
@@ -206,12 +234,13 @@ __device__ inline void step_wide(const Batch& b, const Scalars& c, const Tensor&
 template <int D, int BITS>
 __device__ void step_any(const Batch& b, const Scalars& c, const Tensor& t, int64_t at) {
   using T = typename Elem<D>::type;
-  T* P = static_cast<T*>(t.t.p);
-  const T* G = static_cast<const T*>(t.t.g);
-  const int64_t left = t.t.n - at, blk = at / kBlock;
+  T* P = static_cast<T*>(t.p);
+  const T* G = static_cast<const T*>(t.g);
+  const int64_t left = t.n() - at, blk = at / kBlock;
   const int live = left >= 4 ? 4 : left > 0 ? static_cast<int>(left) : 0;
   float p[4], m[4], v[4];
-  const float ms = BITS == 8 ? t.t.m_scale[blk] : 1, vs = BITS == 8 ? t.t.v_scale[blk] : 1;
+  const float ms = BITS == 8 ? t.m_scale[blk] * b.b1 : b.b1;
+  const float vs = BITS == 8 ? t.v_scale[blk] * b.b2 : b.b2;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     float g = 0;
@@ -220,11 +249,11 @@ __device__ void step_any(const Batch& b, const Scalars& c, const Tensor& t, int6
       p[e] = Elem<D>::up(P[at + e]);
       g = Elem<D>::up(G[at + e]);
       if (BITS == 32) {
-        m[e] = static_cast<const float*>(t.t.m)[at + e];
-        v[e] = static_cast<const float*>(t.t.v)[at + e];
+        m[e] = static_cast<const float*>(t.m)[at + e] * ms;
+        v[e] = static_cast<const float*>(t.v)[at + e] * vs;
       } else {
-        m[e] = __builtin_amdgcn_cvt_f32_fp8(static_cast<const uint8_t*>(t.t.m)[at + e], 0) * ms;
-        v[e] = __builtin_amdgcn_cvt_f32_bf8(static_cast<const uint8_t*>(t.t.v)[at + e], 0) * vs;
+        m[e] = __builtin_amdgcn_cvt_f32_fp8(static_cast<const uint8_t*>(t.m)[at + e], 0) * ms;
+        v[e] = __builtin_amdgcn_cvt_f32_bf8(static_cast<const uint8_t*>(t.v)[at + e], 0) * vs;
       }
     }
     const Moments s = moments(b, m[e], v[e], g);
@@ -234,18 +263,18 @@ __device__ void step_any(const Batch& b, const Scalars& c, const Tensor& t, int6
   }
   unsigned qm[1], qv[1];
   if (BITS == 8)
-    requantize<4, 64>(m, v, c.key, t.t.block0 + blk, at % kBlock, t.t.m_scale + blk,
-                      t.t.v_scale + blk, qm, qv);
+    requantize<4, 64>(m, v, c.key, t.block0 + blk, at % kBlock, t.m_scale + blk,
+                      t.v_scale + blk, qm, qv);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     if (e >= live) continue;
     P[at + e] = Elem<D>::down(p[e]);
     if (BITS == 32) {
-      static_cast<float*>(t.t.m)[at + e] = m[e];
-      static_cast<float*>(t.t.v)[at + e] = v[e];
+      static_cast<float*>(t.m)[at + e] = m[e];
+      static_cast<float*>(t.v)[at + e] = v[e];
     } else {
-      static_cast<uint8_t*>(t.t.m)[at + e] = static_cast<uint8_t>(qm[0] >> (8 * e));
-      static_cast<uint8_t*>(t.t.v)[at + e] = static_cast<uint8_t>(qv[0] >> (8 * e));
+      static_cast<uint8_t*>(t.m)[at + e] = static_cast<uint8_t>(qm[0] >> (8 * e));
+      static_cast<uint8_t*>(t.v)[at + e] = static_cast<uint8_t>(qv[0] >> (8 * e));
     }
   }
 }
@@ -262,7 +291,7 @@ template <int D, int BITS, int PER> __global__ __launch_bounds__(256) void k_ada
   Scalars c = {b.size, b.root, b.key};
   if (b.device) c = {b.device[0], b.device[1], to_bits(b.device[2])};
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  if (PER == 4 && t.wide && chunk + PER * 1024 <= t.t.n) {
+  if (PER == 4 && t.wide() && chunk + PER * 1024 <= t.n()) {
     if constexpr (BITS == 8) {
       step_wide<D, BITS, 16>(b, c, t, chunk + tid * 16);
     } else {
@@ -273,11 +302,13 @@ template <int D, int BITS, int PER> __global__ __launch_bounds__(256) void k_ada
   }
   for (int j = 0; j < PER; ++j) {
     const int64_t first = chunk + (j * 4 + wave) * kBlock;
-    if (first >= t.t.n) return;
-    if (t.wide && first + kBlock <= t.t.n) step_wide<D, BITS, 4>(b, c, t, first + lane * 4);
+    if (first >= t.n()) return;
+    if (t.wide() && first + kBlock <= t.n()) step_wide<D, BITS, 4>(b, c, t, first + lane * 4);
     else step_any<D, BITS>(b, c, t, first + lane * 4);
   }
 }
+
+static_assert(sizeof(Batch) <= 4096, "the arguments of a launch");
 
 struct Corrections {
   float size, root;
@@ -342,12 +373,11 @@ extern "C" int fedtrain_adamw(int dtype, int state_bits, int64_t count,
   hipStream_t st = static_cast<hipStream_t>(stream);
   Batch b;
   b.b1 = static_cast<float>(s->beta1);
-  b.c1 = static_cast<float>(1 - s->beta1);
+  b.c1 = static_cast<float>(1 - s->beta1) * (s->maximize ? -1.0f : 1.0f);
   b.b2 = static_cast<float>(s->beta2);
   b.c2 = static_cast<float>(1 - s->beta2);
   b.decay = static_cast<float>(1 - s->lr * s->weight_decay);
   b.eps = static_cast<float>(s->eps);
-  b.sign = s->maximize ? -1.0f : 1.0f;
   b.device = nullptr;
   b.size = b.root = 0;
   b.key = 0;
@@ -370,9 +400,16 @@ extern "C" int fedtrain_adamw(int dtype, int state_bits, int64_t count,
       const int64_t groups = (t.n + per * 1024 - 1) / (per * 1024);
       if (grid + groups > INT32_MAX) break;
       Tensor& at = b.at[b.count++];
-      at.t = t;
+      at.p = t.p;
+      at.g = t.g;
+      at.m = t.m;
+      at.v = t.v;
+      at.m_scale = t.m_scale;
+      at.v_scale = t.v_scale;
       at.first = static_cast<int>(grid);
-      at.wide = aligned(t.p, 16) && aligned(t.g, 16) && aligned(t.m, 16) && aligned(t.v, 16);
+      at.block0 = static_cast<unsigned>(t.block0);
+      at.n_wide = t.n * 2 + (aligned(t.p, 16) && aligned(t.g, 16) && aligned(t.m, 16) &&
+                             aligned(t.v, 16));
       grid += groups;
     }
     if (!b.count) break;

@@ -69,7 +69,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
                betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                weight_decay: float = 1e-2, maximize: bool = False, seed: int = 0,
                first_blocks: Optional[Sequence[int]] = None) -> None:
-    """One AdamW step of all ``params``, in place, in one launch for each 40
+    """One AdamW step of all ``params``, in place, in one launch for each 62
     tensors::
 
         m = b1 m + (1 - b1) g            v = b2 v + (1 - b2) g g
