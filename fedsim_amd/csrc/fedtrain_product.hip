@@ -396,47 +396,45 @@ struct Plan {
   int64_t tiles_m, tiles_n;  // tiles_m: of one group (grad weight), or slots
   int high;                  // rows of tiles in a band, see place()
   int splits;                // parts of k; over 1, C is f32 partial sums in the workspace
-  int wide;                  // 1: eight neighbouring values of C's operands are 16-byte aligned
 };
 
 // ---------------------------------------------------------------------------
 // what becomes of the sums
 // ---------------------------------------------------------------------------
-// Eight neighbouring values in memory, as one or two accesses of 16 bytes; n of
-// them where they are not `wide`.
-template <class T> struct __attribute__((aligned(16))) Eight {
-  T v[8];
-};
-
-template <int D> __device__ inline void read8(const void* p, int64_t at, int n, bool wide,
-                                              float* to) {
+// n <= 8 neighbouring values in memory; all eight are one or two accesses of 16
+// bytes, which need no alignment beyond the values' own.
+template <int D> __device__ inline void read8(const void* p, int64_t at, int n, float* to) {
   using T = typename Elem<D>::type;
   const T* x = static_cast<const T*>(p) + at;
-  if (wide) {
-    const Eight<T> f = *reinterpret_cast<const Eight<T>*>(x);
+  if (n >= 8) {
+    T f[8];
+    __builtin_memcpy(f, x, sizeof(f));
 #pragma unroll
-    for (int e = 0; e < 8; ++e) to[e] = Elem<D>::up(f.v[e]);
+    for (int e = 0; e < 8; ++e) to[e] = Elem<D>::up(f[e]);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) to[e] = e < n ? Elem<D>::up(x[e]) : 0.0f;
   }
 }
 
-template <int D> __device__ inline void write8(void* p, int64_t at, int n, bool wide,
-                                               const float* v) {
+template <int D> __device__ inline void write8(void* p, int n, const float* v) {
   using T = typename Elem<D>::type;
-  T* x = static_cast<T*>(p) + at;
-  if (wide) {
-    Eight<T> f;
+  T* x = static_cast<T*>(p);
+  if (n >= 8) {
+    T f[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f.v[e] = Elem<D>::down(v[e]);
-    *reinterpret_cast<Eight<T>*>(x) = f;
+    for (int e = 0; e < 8; ++e) f[e] = Elem<D>::down(v[e]);
+    __builtin_memcpy(x, f, sizeof(f));
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (e < n) x[e] = Elem<D>::down(v[e]);
   }
 }
+
+struct __attribute__((aligned(16))) Eight {
+  float v[8];
+};
 
 // Where eight neighbouring columns of C are written, row by row.
 template <int D, int FORM> struct Out {
@@ -445,17 +443,17 @@ template <int D, int FORM> struct Out {
   const T* res;
   float bias[8];
   int n;
-  bool wide, held;  // held: by a group; other rows get their residual
+  bool held;  // by a group; other rows get their residual
 
-  __device__ Out(const Args& a, bool wide_, int group, int64_t row, int64_t col, int64_t n_)
-      : n(static_cast<int>(n_ < 8 ? n_ : 8)), wide(wide_ && n_ >= 8), held(group >= 0) {
+  __device__ Out(const Args& a, int group, int64_t row, int64_t col, int64_t n_)
+      : n(static_cast<int>(n_ < 8 ? n_ : 8)), held(group >= 0) {
     const int64_t first = FORM == FEDTRAIN_GRAD_WEIGHT ? group * a.c_group : 0;
     c = static_cast<T*>(a.c) + first + row * a.ldc + col;
     if constexpr (FORM == FEDTRAIN_FORWARD) {
       z = a.z ? static_cast<T*>(a.z) + row * a.ldz + col : nullptr;
       res = a.res ? static_cast<const T*>(a.res) + row * a.ldr + col : nullptr;
       if (a.bias && held && n > 0) {
-        read8<D>(a.bias, group * a.bias_group + col, n, wide, bias);
+        read8<D>(a.bias, group * a.bias_group + col, n, bias);
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) bias[e] = 0;
@@ -475,19 +473,19 @@ template <int D, int FORM> struct Out {
     if constexpr (FORM == FEDTRAIN_FORWARD) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += bias[e];
-      if (z) write8<D>(z, 0, n, wide, v);
+      if (z) write8<D>(z, n, v);
       if (held) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = act_value<D, ACT>(v[e]);
       }
       if (res) {
         float r[8];
-        read8<D>(res, 0, n, wide, r);
+        read8<D>(res, 0, n, r);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += r[e];
       }
     }
-    write8<D>(c, 0, n, wide, v);
+    write8<D>(c, n, v);
   }
 };
 
@@ -773,7 +771,7 @@ void k_product(Args a, Plan plan) {
   auto spot = [](int row, int four) { return row * (LINE / 4) + (four ^ (row & (LINE / 4 - 1))); };
   const int c8 = lane % EIGHTS, c = wn + c8 * 8, n = static_cast<int>(cols) - c;
   int r = wm + lane / EIGHTS;
-  Out<D, FORM> out(a, plan.wide, group, row0 + r, col0 + c, n);
+  Out<D, FORM> out(a, group, row0 + r, col0 + c, n);
 #pragma unroll
   for (int i0 = 0; i0 < S::MI; i0 += FIT) {
 #pragma unroll
@@ -788,10 +786,10 @@ void k_product(Args a, Plan plan) {
         float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
         if (r < rows && n > 0) {
           if (plan.splits > 1) {
-            Eight<float> f;
+            Eight f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) f.v[e] = v[e];
-            *reinterpret_cast<Eight<float>*>(partial + r * width + col0 + c) = f;
+            *reinterpret_cast<Eight*>(partial + r * width + col0 + c) = f;
           } else {
             out.template put<decltype(act)::value>(v);
           }
@@ -814,7 +812,7 @@ template <int D, int FORM> __global__ __launch_bounds__(256) void k_join(Args a,
   float v[8] = {};
 #pragma unroll 4
   for (int s = 0; s < plan.splits; ++s) {
-    const Eight<float> f = *reinterpret_cast<const Eight<float>*>(P + s * a.m * width);
+    const Eight f = *reinterpret_cast<const Eight*>(P + s * a.m * width);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += f.v[e];
   }
@@ -829,31 +827,83 @@ template <int D, int FORM> __global__ __launch_bounds__(256) void k_join(Args a,
     if (group < 0)
       for (int e = 0; e < 8; ++e) v[e] = 0;
   }
-  const Out<D, FORM> out(a, plan.wide, group, row, col, a.n - col);
+  const Out<D, FORM> out(a, group, row, col, a.n - col);
   by_act(FORM == FEDTRAIN_FORWARD ? a.act : 0,
          [&](auto act) { out.template put<decltype(act)::value>(v); });
 }
 
-// dz = dy act'(z): one pass, eight values a thread where rows allow it
-template <int D, int ACT, int V>
+// The forward product of a few rows: the weights are read once, at the rate of
+// memory, and each lane adds up its part of k by itself.  A wave takes COLS columns
+// and one of PARTS parts of k, which its workgroup's other waves complete.
+template <int D, int ROWS, int COLS, int PARTS>
+__global__ __launch_bounds__(256) void k_few_rows(Args a) {
+  using T = typename Elem<D>::type;
+  constexpr int TEAMS = 4 / PARTS;
+  __shared__ float part[4][ROWS * COLS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int team = wave / PARTS, mine = wave % PARTS;
+  const int64_t col0 = (static_cast<int64_t>(blockIdx.x) * TEAMS + team) * COLS;
+  const T* X = static_cast<const T*>(a.a);
+  const T* W[COLS];
+#pragma unroll
+  for (int c = 0; c < COLS; ++c)  // columns past the last read the last
+    W[c] = static_cast<const T*>(a.b) + (col0 + c < a.n ? col0 + c : a.n - 1) * a.ldb;
+  float acc[ROWS][COLS] = {};
+  auto step = [&](int64_t k, int n) {
+    float w[COLS][8];
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) read8<D>(W[c], k, n, w[c]);
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      float x[8];
+      read8<D>(X, (r < a.m ? r : 0) * a.lda + k, n, x);
+#pragma unroll
+      for (int c = 0; c < COLS; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[r][c] = __builtin_fmaf(x[e], w[c][e], acc[r][c]);
+    }
+  };
+  int64_t k = (mine * 64 + lane) * 8;
+#pragma unroll 2
+  for (; k + 8 <= a.k; k += PARTS * 64 * 8) step(k, 8);
+  if (k < a.k) step(k, static_cast<int>(a.k - k));
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) {
+#pragma unroll
+      for (int s = 32; s; s >>= 1) acc[r][c] += __shfl_xor(acc[r][c], s);
+      if (lane == 0) part[wave][r * COLS + c] = acc[r][c];
+    }
+  __syncthreads();
+  if (threadIdx.x >= TEAMS * ROWS * COLS) return;
+  const int t = threadIdx.x / (ROWS * COLS), i = threadIdx.x % (ROWS * COLS);
+  const int r = i / COLS;
+  const int64_t col = (static_cast<int64_t>(blockIdx.x) * TEAMS + t) * COLS + i % COLS;
+  if (r >= a.m || col >= a.n) return;
+  float v[8] = {};
+  for (int s = 0; s < PARTS; ++s) v[0] += part[t * PARTS + s][i];
+  const Out<D, FEDTRAIN_FORWARD> out(a, 0, r, col, 1);
+  by_act(a.act, [&](auto act) { out.template put<decltype(act)::value>(v); });
+}
+
+// dz = dy act'(z): one pass, eight values of a row a thread, at any alignment
+template <int D, int ACT>
 __global__ __launch_bounds__(256) void k_act_backward(int64_t rows, int64_t cols, const void* dy,
                                                       int64_t lddy, const void* z, int64_t ldz,
                                                       void* dz, int64_t lddz) {
   using T = typename Elem<D>::type;
-  struct __attribute__((aligned(V * sizeof(T)))) Vec {
-    T v[V];
-  };
-  const int64_t per = cols / V;
+  const int64_t per = (cols + 7) / 8;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (i >= rows * per) return;
-  const int64_t r = i / per, c = i % per * V;
-  const Vec g = *reinterpret_cast<const Vec*>(static_cast<const T*>(dy) + r * lddy + c);
-  const Vec x = *reinterpret_cast<const Vec*>(static_cast<const T*>(z) + r * ldz + c);
-  Vec out;
+  const int64_t r = rows == 1 ? 0 : i / per, c = (i - r * per) * 8;
+  const int n = static_cast<int>(cols - c < 8 ? cols - c : 8);
+  float g[8], x[8];
+  read8<D>(dy, r * lddy + c, n, g);
+  read8<D>(z, r * ldz + c, n, x);
 #pragma unroll
-  for (int e = 0; e < V; ++e)
-    out.v[e] = Elem<D>::down(Elem<D>::up(g.v[e]) * act_slope<D, ACT>(Elem<D>::up(x.v[e])));
-  *reinterpret_cast<Vec*>(static_cast<T*>(dz) + r * lddz + c) = out;
+  for (int e = 0; e < 8; ++e) g[e] *= act_slope<D, ACT>(x[e]);
+  write8<D>(static_cast<T*>(dz) + r * lddz + c, n, g);
 }
 
 // ---------------------------------------------------------------------------
@@ -906,14 +956,6 @@ bool in_eights(const Args& a) {
          a.lda < (1 << 21) && a.ldb < (1 << 21);
 }
 
-// Whether eight neighbours of C and what goes into it are 16-byte accesses.
-bool out_in_eights(const Args& a) {
-  const int64_t n = a.dtype == FEDTRAIN_F32 ? 4 : 8;
-  return aligned(a.c, 16) && aligned(a.z, 16) && aligned(a.res, 16) && aligned(a.bias, 16) &&
-         a.ldc % n == 0 && a.c_group % n == 0 && (!a.z || a.ldz % n == 0) &&
-         (!a.res || a.ldr % n == 0) && (!a.bias || a.bias_group % n == 0);
-}
-
 enum class Size { Large, Middle, Small };
 
 struct Choice {
@@ -930,8 +972,8 @@ struct Kind {
   double first, alone, full;
 };
 
-const Kind kDirect[] = {{Size::Large, 256, 256, 1, 12.0, 1.7, 1.7},
-                        {Size::Middle, 128, 128, 2, 6.0, 0.75, 1.2},
+const Kind kDirect[] = {{Size::Large, 256, 256, 1, 13.0, 1.7, 1.7},
+                        {Size::Middle, 128, 128, 2, 4.0, 0.75, 1.2},
                         {Size::Small, 64, 64, 5, 4.0, 0.45, 1.1}};
 const Kind kThrough[] = {{Size::Middle, 128, 128, 2, 6.0, 1.2, 1.6},
                          {Size::Small, 64, 64, 4, 4.0, 1.1, 1.4}};
@@ -976,7 +1018,17 @@ Choice choose(const Args& a) {
   return best;
 }
 
+// Up to 4 rows of one weight matrix, while reading the weights costs more than the
+// vector unit's products.  4096 x 4096: one bf16 row 8.8 us, on the matrix unit
+// 12; two 12.1 and 11.9, four 15.4 and 11.9; four f32 rows 20 and 25.  784 x 200:
+// 4 to 5 us, in place of 8 (bf16) and 11 (f32) by parts of k and their sum.
+bool few_rows(const Args& a) {
+  return a.form == FEDTRAIN_FORWARD && !a.groups && a.m <= 4 &&
+         (a.dtype == FEDTRAIN_F32 || a.m == 1 || a.m * a.n * a.k <= 1 << 24);
+}
+
 int64_t workspace(const Args& a) {
+  if (few_rows(a)) return 0;
   const int s = choose(a).splits;
   if (s < 2) return 0;
   return static_cast<int64_t>(s) * a.m * ((a.n + 7) / 8 * 8 + (a.colsum ? 8 : 0)) * 4;
@@ -985,7 +1037,6 @@ int64_t workspace(const Args& a) {
 template <int D, int FORM, class S> int go(const Args& a, int splits, hipStream_t s) {
   Plan p;
   p.splits = splits;
-  p.wide = out_in_eights(a);
   p.tiles_n = a.n ? (a.n + S::BN - 1) / S::BN : 1;
   int64_t all;
   if (FORM == FEDTRAIN_GRAD_WEIGHT) {
@@ -1026,6 +1077,26 @@ template <int D, int FORM, class S> int go(const Args& a, int splits, hipStream_
   return launched();
 }
 
+template <int D, int ROWS, int COLS, int PARTS> int go_few_rows(const Args& a, hipStream_t s) {
+  constexpr int64_t each = 4 / PARTS * COLS;
+  hipLaunchKernelGGL((k_few_rows<D, ROWS, COLS, PARTS>),
+                     dim3(static_cast<unsigned>((a.n + each - 1) / each)), dim3(256), 0, s, a);
+  return launched();
+}
+
+template <int D, int ROWS> int go_few_rows(const Args& a, hipStream_t s) {
+  // 2048 waves or more, two to a SIMD
+  if (a.n >= 8192) return go_few_rows<D, ROWS, 4, 1>(a, s);
+  if (a.n >= 4096) return go_few_rows<D, ROWS, 4, 2>(a, s);
+  return go_few_rows<D, ROWS, 2, 4>(a, s);
+}
+
+template <int D> int run_few_rows(const Args& a, hipStream_t s) {
+  if (a.m <= 1) return go_few_rows<D, 1>(a, s);
+  if (a.m <= 2) return go_few_rows<D, 2>(a, s);
+  return go_few_rows<D, 4>(a, s);
+}
+
 template <int D, int FORM> int run(const Args& a, hipStream_t s) {
   const Choice c = choose(a);
   if (c.splits > 1 && (!a.workspace || !aligned(a.workspace, 16) ||
@@ -1046,6 +1117,7 @@ template <int D, int FORM> int run(const Args& a, hipStream_t s) {
 }
 
 template <int D> int run(const Args& a, hipStream_t s) {
+  if (few_rows(a)) return run_few_rows<D>(a, s);
   if (a.form == FEDTRAIN_FORWARD) return run<D, FEDTRAIN_FORWARD>(a, s);
   if (a.form == FEDTRAIN_GRAD_INPUT) return run<D, FEDTRAIN_GRAD_INPUT>(a, s);
   return run<D, FEDTRAIN_GRAD_WEIGHT>(a, s);
@@ -1061,19 +1133,17 @@ struct Slope {
   int64_t lddz;
 };
 
-template <int D, int ACT, int V> int slope(const Slope& x, hipStream_t s) {
-  const int64_t n = x.rows * (x.cols / V);
+template <int D, int ACT> int slope(const Slope& given, hipStream_t s) {
+  Slope x = given;
+  if (x.lddy == x.cols && x.ldz == x.cols && x.lddz == x.cols) {  // one long row
+    x.cols *= x.rows;
+    x.rows = 1;
+  }
+  const int64_t n = x.rows * ((x.cols + 7) / 8);
   if (n > static_cast<int64_t>(INT32_MAX) * 256) return FEDTRAIN_EINVAL;
-  hipLaunchKernelGGL((k_act_backward<D, ACT, V>), dim3(static_cast<unsigned>((n + 255) / 256)),
+  hipLaunchKernelGGL((k_act_backward<D, ACT>), dim3(static_cast<unsigned>((n + 255) / 256)),
                      dim3(256), 0, s, x.rows, x.cols, x.dy, x.lddy, x.z, x.ldz, x.dz, x.lddz);
   return launched();
-}
-
-template <int D, int ACT> int slope(const Slope& x, hipStream_t s) {
-  constexpr int V = D == FEDTRAIN_F32 ? 4 : 8;
-  const bool wide = aligned(x.dy, 16) && aligned(x.z, 16) && aligned(x.dz, 16) &&
-                    x.cols % V == 0 && x.lddy % V == 0 && x.ldz % V == 0 && x.lddz % V == 0;
-  return wide ? slope<D, ACT, V>(x, s) : slope<D, ACT, 1>(x, s);
 }
 
 template <int D> int slope(int act, const Slope& x, hipStream_t s) {
