@@ -59,6 +59,10 @@ SIGNATURES = {
     "fedtrain_abi_version": (ctypes.c_int, []),
     "fedtrain_strerror": (ctypes.c_char_p, [ctypes.c_int]),
     "fedtrain_product_workspace": (ctypes.c_int64, [ctypes.POINTER(ProductArgs)]),
+    "fedtrain_product_plan": (
+        ctypes.c_int,
+        [ctypes.POINTER(ProductArgs)] + [ctypes.POINTER(ctypes.c_int)] * 3,
+    ),
     "fedtrain_product": (ctypes.c_int, [ctypes.POINTER(ProductArgs), ctypes.c_void_p]),
     "fedtrain_act_backward": (
         ctypes.c_int,

@@ -11,6 +11,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
 #include <string>
 #include <tuple>
 #include <vector>
@@ -407,6 +408,13 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& ms,
   for (size_t i = 0; i < n; ++i) {
     sizes[i] = params[i].numel();
     blocks[i] = (sizes[i] + kStateBlock - 1) / kStateBlock;
+  }
+  {
+    std::vector<const void*> places(n);
+    for (size_t i = 0; i < n; ++i) places[i] = sizes[i] ? params[i].const_data_ptr() : nullptr;
+    std::sort(places.begin(), places.end());
+    for (size_t i = 1; i < n; ++i)
+      TORCH_CHECK_VALUE(!places[i] || places[i] != places[i - 1], "a parameter is given twice");
   }
   const bool eight = m_scales.has_value();
   TORCH_CHECK_VALUE(eight == v_scales.has_value(),

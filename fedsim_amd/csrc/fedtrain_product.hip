@@ -1037,7 +1037,8 @@ Choice choose(const Args& a) {
 // 4 to 5 us, in place of 8 (bf16) and 11 (f32) by parts of k and their sum.
 bool few_rows(const Args& a) {
   return a.form == FEDTRAIN_FORWARD && !a.groups && a.m <= 4 &&
-         (a.dtype == FEDTRAIN_F32 || a.m == 1 || a.m * a.n * a.k <= 1 << 24);
+         (a.dtype == FEDTRAIN_F32 || a.m == 1 ||
+          static_cast<double>(a.m) * a.n * a.k <= 1 << 24);
 }
 
 int64_t workspace(const Args& a) {
@@ -1190,6 +1191,20 @@ const char* fedtrain_strerror(int status) {
 
 int64_t fedtrain_product_workspace(const Args* args) {
   return valid(args) ? workspace(*args) : FEDTRAIN_EINVAL;
+}
+
+int fedtrain_product_plan(const Args* args, int* rows, int* cols, int* parts) {
+  if (!valid(args) || !rows || !cols || !parts) return FEDTRAIN_EINVAL;
+  if (few_rows(*args)) {
+    *rows = static_cast<int>(args->m);
+    *cols = *parts = 1;
+    return 0;
+  }
+  const Choice c = choose(*args);
+  *rows = c.size == Size::Large ? 256 : c.size == Size::Middle ? 128 : 64;
+  *cols = c.size == Size::Small && args->dtype == FEDTRAIN_F32 ? 128 : *rows;
+  *parts = c.splits;
+  return 0;
 }
 
 int fedtrain_product(const Args* args, void* stream) {

@@ -120,6 +120,9 @@ class AdamW(torch.optim.Optimizer):
                 n = st["step"]
                 break
         if n is None:
+            if torch.cuda.is_current_stream_capturing():  # a replay would start again
+                raise RuntimeError("take a step before capturing one: the first puts the count "
+                                   "on the device")
             known = [int(self.state[p]["step"]) for p in group["params"] if self.state.get(p)
                      and p.device == dev]
             n = torch.full((1,), max(known, default=0), dtype=torch.int64, device=dev)

@@ -80,6 +80,10 @@ const char* fedtrain_strerror(int status);
 int64_t fedtrain_product_workspace(const fedtrain_product_args* args);
 int fedtrain_product(const fedtrain_product_args* args, void* stream);
 
+/* The tile of C a workgroup of that call takes (1 column: the kernel for a few
+ * rows), and the parts k is taken in. */
+int fedtrain_product_plan(const fedtrain_product_args* args, int* rows, int* cols, int* parts);
+
 /* dz = dy act'(z), [rows, cols] with row strides; relu takes z or act(z). */
 int fedtrain_act_backward(int dtype, int act, int64_t rows, int64_t cols, const void* dy,
                           int64_t lddy, const void* z, int64_t ldz, void* dz, int64_t lddz,

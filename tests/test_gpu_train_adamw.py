@@ -329,6 +329,30 @@ def test_capture_refusals():
     opt.step()
 
 
+def test_a_loaded_state_takes_a_step_before_a_capture():
+    """A loaded state's step is the host's number: a graph that put it on the
+    device would start from it at every replay."""
+    from fedsim_amd.optim import AdamW
+
+    p = torch.nn.Parameter(torch.ones(10, device=DEV))
+    p.grad = torch.ones_like(p)
+    opt = AdamW([p], capturable=True)
+    opt.step()
+    opt.load_state_dict(opt.state_dict())
+    with pytest.raises(RuntimeError, match="before capturing"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    torch.cuda.synchronize()
+    opt.step()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        opt.step()
+    for k in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert int(opt.state[p]["step"]) == 3 + k
+
+
 def test_same_bits_every_time_and_on_another_stream():
     from fedsim_amd.train_ops import adamw_step
 

@@ -35,12 +35,13 @@ def _up(t):
     return None if t is None else t.double()
 
 
-def _check(x, w, b, r, dy, act, edges=None, offsets=None, place=lambda t: t):
-    """Forward and backward of the operator against the definition; ``place``
-    lays a device tensor out in memory."""
+def _check(x, w, b, r, dy, act, edges=None, offsets=None, place=lambda t: t, on="cpu"):
+    """Forward and backward of the operator against the definition, which is
+    worked out ``on`` a device; ``place`` lays a device tensor out in memory."""
     from fedsim_amd.functional import grouped_linear, linear_act
 
-    want = R.product(_up(x), _up(w), _up(b), _up(r), act, x.dtype, _up(dy), edges)
+    want = R.product(*(None if t is None else t.to(on).double() for t in (x, w, b, r)),
+                     act, x.dtype, dy.to(on).double(), edges)
     leaves = [None if t is None else place(t.to(DEV)).requires_grad_(True) for t in (x, w, b, r)]
     X, W, B, Rr = leaves
     if edges is None:
@@ -101,6 +102,17 @@ def test_linear_large_tiles(shape, dtype):
     """Sizes that fill the widest tiles, with and without a remainder."""
     _check(*_case(*shape, dtype, 2), "gelu")
     _check(*_case(*shape, dtype, 3, bias=False, residual=False), "none")
+
+
+@pytest.mark.parametrize("dtype,shape", [
+    (torch.bfloat16, (4001, 3976, 4008)), (torch.float16, (4001, 3976, 4008)),
+    (torch.bfloat16, (2600, 2051, 2049)), (torch.float16, (2600, 2051, 2049)),
+    (torch.float32, (2600, 2051, 2049))], ids=str)
+def test_linear_widest_tiles(dtype, shape):
+    """Sizes at which each product takes the widest tiles there are for its type
+    and alignment, with remainders."""
+    _check(*_case(*shape, dtype, 4), "gelu", on=DEV)
+    _check(*_case(*shape, dtype, 5, bias=False, residual=False), "none", on=DEV)
 
 
 def _padded(t):
@@ -203,6 +215,18 @@ def test_grouped_large_tiles(i, o, dtype):
         edges.append(edges[-1] + n)
     x, w, b, r, dy = _case(edges[-1], i, o, dtype, 3, len(sizes))
     _check(x, w, b, r, dy, "silu", edges, torch.tensor(edges, device=DEV))
+
+
+@pytest.mark.parametrize("dtype,i,o", [
+    (torch.bfloat16, 1544, 1544), (torch.float16, 1544, 1544), (torch.bfloat16, 1535, 1281),
+    (torch.float16, 1535, 1281), (torch.float32, 1535, 1281)], ids=str)
+def test_grouped_widest_tiles(dtype, i, o):
+    """As test_linear_widest_tiles, with a group of two thirds of the rows, an empty
+    one, one of 70 and rows of no group."""
+    edges = [1, 1500, 1500, 1570, 8191]
+    N = 8192
+    x, w, b, r, dy = _case(N, i, o, dtype, 12, 4)
+    _check(x, w, b, r, dy, "silu", edges, torch.tensor(edges, device=DEV), on=DEV)
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)

@@ -72,6 +72,52 @@ def test_product_without_work(lib):
         assert lib.fedtrain_product(ctypes.byref(_args(**kw)), None) == 0
 
 
+def _plan(lib, **kw):
+    got = [ctypes.c_int() for _ in range(3)]
+    assert lib.fedtrain_product_plan(ctypes.byref(_args(**kw)),
+                                     *(ctypes.byref(g) for g in got)) == 0
+    return tuple(g.value for g in got)
+
+
+# (dtype, aligned, form, sizes) -> the tile and whether k is taken in parts
+PLANS = [
+    (1, True, 0, (4001, 4008, 3976), (256, 256), False),
+    (2, True, 1, (4001, 3976, 4008), (256, 256), False),
+    (1, True, 2, (4008, 3976, 4001), (256, 256), False),
+    (2, True, 0, (2048, 2048, 520), (128, 128), False),
+    (1, True, 1, (4000, 520, 4008), (128, 128), True),
+    (1, True, 2, (1024, 2304, 264), (128, 128), False),
+    (1, True, 0, (300, 520, 136), (64, 64), False),
+    (1, True, 1, (64, 200, 4096), (64, 64), True),
+    (2, False, 0, (2049, 2047, 517), (128, 128), False),
+    (1, False, 2, (300, 261, 135), (64, 64), False),
+    (1, False, 0, (40, 33, 5001), (64, 64), True),
+    (0, True, 0, (3000, 2500, 300), (128, 128), False),
+    (0, False, 1, (700, 900, 100), (64, 128), False),
+    (0, True, 2, (500, 100, 9000), (64, 128), True),
+    (0, False, 0, (4, 300, 1000), (4, 1), False),
+    (1, True, 0, (1, 4096, 4096), (1, 1), False),
+]
+
+
+@pytest.mark.parametrize("dtype,aligned,form,mnk,tile,parts", PLANS, ids=str)
+def test_plans(lib, dtype, aligned, form, mnk, tile, parts):
+    """Which kernel takes what: each of them is taken somewhere."""
+    m, n, k = mnk
+    lda, ldb = (k, k) if form == 0 else (k, n) if form == 1 else (m, n)
+    got = _plan(lib, dtype=dtype, form=form, m=m, n=n, k=k, lda=lda, ldb=ldb, ldc=n,
+                a=64 if aligned else 68)
+    assert got[:2] == tile and (got[2] > 1) == parts, got
+
+
+def test_plan_refusals(lib):
+    i = ctypes.c_int()
+    r = ctypes.byref(i)
+    assert lib.fedtrain_product_plan(ctypes.byref(_args(dtype=9)), r, r, r) == E
+    assert lib.fedtrain_product_plan(ctypes.byref(_args()), None, r, r) == E
+    assert lib.fedtrain_product_plan(None, r, r, r) == E
+
+
 def test_act_backward_refusals(lib):
     f = lib.fedtrain_act_backward
     ok = [0, 1, 2, 4, 64, 4, 64, 4, 64, 4, None]
@@ -206,6 +252,7 @@ def test_functions_refuse_what_does_not_fit():
                 lambda: train_ops.adamw_step([p], [p], [p], [p], step=t(1), lr=1e-3),
                 lambda: train_ops.adamw_step([p], [p], [p], [p], step=1, lr=1e-3,
                                              betas=(0.9, 1.0)),
+                lambda: train_ops.adamw_step([p, p], [p, p], [p, p], [p, p], **ok),
                 lambda: train_ops.adamw_step([p], [p], [p], [p], first_blocks=[], **ok)):
         with pytest.raises(ValueError):
             bad()

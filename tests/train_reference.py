@@ -1,5 +1,4 @@
-"""The dense training operators from their definitions, in 64 bits on the CPU,
-with bounds on how far a float32-summed kernel may be from them.
+"""The dense training operators from their definitions, in 64 bits, with bounds on how far a float32-summed kernel may be from them.
 
 Bounds.  A value stored in a type t is off by at most h = eps(t) / 2 relative to
 it.  A sum of K products in float32, in any order, is off by at most
@@ -48,7 +47,7 @@ def sum_error(K, S):
 
 
 def product(x, w, b, r, kind, dtype, dy=None, edges=None):
-    """{name: (value, bound)} of y, dx, dw, db for float64 CPU tensors;
+    """{name: (value, bound)} of y, dx, dw, db for float64 tensors of one device;
     ``edges``: the groups' row bounds (w and b then have a group dimension)."""
     h, t = HALF[dtype], TINY[dtype]
     N, o = x.shape[0], w.shape[-2]
@@ -56,13 +55,13 @@ def product(x, w, b, r, kind, dtype, dy=None, edges=None):
     if not grouped:
         edges, w, b = [0, N], w[None], None if b is None else b[None]
     G = len(edges) - 1
-    y = torch.zeros(N, o, dtype=torch.float64) if r is None else r.clone()
+    y = torch.zeros(N, o, dtype=torch.float64, device=x.device) if r is None else r.clone()
     ey = h * y.abs()
     out = {}
     if dy is not None:
         dx, edx = torch.zeros_like(x), torch.zeros_like(x)
         dw, edw = torch.zeros_like(w), torch.zeros_like(w)
-        db = torch.zeros(G, o, dtype=torch.float64)
+        db = torch.zeros(G, o, dtype=torch.float64, device=x.device)
         edb = torch.zeros_like(db)
     for g in range(G):
         s = slice(edges[g], max(edges[g], edges[g + 1]))
@@ -114,7 +113,7 @@ def product(x, w, b, r, kind, dtype, dy=None, edges=None):
 
 def close(got, want, what=""):
     value, bound = want
-    got = got.detach().double().cpu()
+    got = got.detach().double().to(value.device)
     assert got.shape == value.shape, (what, got.shape, value.shape)
     if not got.numel():
         return
