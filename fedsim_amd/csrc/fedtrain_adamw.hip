@@ -365,7 +365,7 @@ extern "C" int fedtrain_adamw(int dtype, int state_bits, int64_t count,
     if (state_bits == 8 &&
         (!t.m_scale || !t.v_scale || !aligned(t.m_scale, 4) || !aligned(t.v_scale, 4)))
       return FEDTRAIN_EINVAL;
-    if (t.n > int64_t{1} << 40) return FEDTRAIN_EINVAL;
+    if (t.n > kMostGroups * 1024) return FEDTRAIN_EINVAL;
     total += t.n;
   }
   // below 4 workgroups of 1024 elements a compute unit the smaller ones win
@@ -398,7 +398,7 @@ extern "C" int fedtrain_adamw(int dtype, int state_bits, int64_t count,
       const fedtrain_adamw_tensor& t = tensors[i];
       if (!t.n) continue;
       const int64_t groups = (t.n + per * 1024 - 1) / (per * 1024);
-      if (grid + groups > INT32_MAX) break;
+      if (grid + groups > kMostGroups) break;
       Tensor& at = b.at[b.count++];
       at.p = t.p;
       at.g = t.g;

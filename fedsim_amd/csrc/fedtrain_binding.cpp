@@ -55,8 +55,9 @@ void require(const Tensor& t, const char* name, const Tensor& like) {
                     t.device());
 }
 
-// The last dimension's elements next to each other.
+// The last dimension's elements next to each other, as they are in memory.
 Tensor rows(const Tensor& t) {
+  if (t.is_neg()) return t.resolve_neg().contiguous();
   return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
 }
 
@@ -336,6 +337,9 @@ struct Product : torch::autograd::Function<Product> {
 
 Tensor product(const Tensor& x, const Tensor& w, const optional<Tensor>& b,
                const optional<Tensor>& r, const optional<Tensor>& offsets, int act) {
+  auto dual = [](const Tensor& t) { return t._fw_grad(0).defined(); };
+  TORCH_CHECK_NOT_IMPLEMENTED(!dual(x) && !dual(w) && !(b && dual(*b)) && !(r && dual(*r)),
+                              "linear_act and grouped_linear have no forward-mode derivative");
   if (at::GradMode::is_enabled() &&
       (x.requires_grad() || w.requires_grad() || wants(b) || wants(r)))
     return Product::apply(x, w, b, r, offsets, act);
@@ -382,11 +386,25 @@ void same(const Tensors& ts, const char* name, at::ScalarType type, const at::De
   for (size_t i = 0; i < ts.size(); ++i) {
     const Tensor& t = ts[i];
     TORCH_CHECK_VALUE(t.scalar_type() == type && t.device() == d && t.numel() == sizes[i] &&
-                          t.is_contiguous(),
+                          t.is_contiguous() && !t.is_neg(),
                       name, "[", i, "] must be a contiguous ", type, " tensor of ", sizes[i],
                       " elements on ", d, ", got ", t.scalar_type(), " ", t.sizes(), " on ",
                       t.device());
   }
+}
+
+// Two workgroups would write the same elements.
+void apart(const Tensors& ts, const char* name) {
+  std::vector<std::pair<uintptr_t, uintptr_t>> at;
+  at.reserve(ts.size());
+  for (const Tensor& t : ts) {
+    const auto p = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+    if (t.numel()) at.emplace_back(p, p + t.nbytes());
+  }
+  std::sort(at.begin(), at.end());
+  for (size_t i = 1; i < at.size(); ++i)
+    TORCH_CHECK_VALUE(at[i].first >= at[i - 1].second, "two of ", name,
+                      " share memory: a tensor is given once");
 }
 
 void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& ms,
@@ -409,13 +427,6 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& ms,
     sizes[i] = params[i].numel();
     blocks[i] = (sizes[i] + kStateBlock - 1) / kStateBlock;
   }
-  {
-    std::vector<const void*> places(n);
-    for (size_t i = 0; i < n; ++i) places[i] = sizes[i] ? params[i].const_data_ptr() : nullptr;
-    std::sort(places.begin(), places.end());
-    for (size_t i = 1; i < n; ++i)
-      TORCH_CHECK_VALUE(!places[i] || places[i] != places[i - 1], "a parameter is given twice");
-  }
   const bool eight = m_scales.has_value();
   TORCH_CHECK_VALUE(eight == v_scales.has_value(),
                     "exp_avg_scales and exp_avg_sq_scales are given together");
@@ -426,6 +437,13 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& ms,
   if (eight) {
     same(*m_scales, "exp_avg_scales", at::kFloat, d, blocks);
     same(*v_scales, "exp_avg_sq_scales", at::kFloat, d, blocks);
+  }
+  apart(params, "params");
+  apart(ms, "exp_avgs");
+  apart(vs, "exp_avg_sqs");
+  if (eight) {
+    apart(*m_scales, "exp_avg_scales");
+    apart(*v_scales, "exp_avg_sq_scales");
   }
   TORCH_CHECK_VALUE(!first_blocks || first_blocks->size() == n, "first_blocks: one for each of ",
                     n, " parameters");

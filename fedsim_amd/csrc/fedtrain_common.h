@@ -33,6 +33,9 @@ template <> struct Elem<FEDTRAIN_F16> {
 
 inline bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 
+// workgroups of 256 in a launch: its threads are counted in 32 bits
+constexpr int64_t kMostGroups = UINT32_MAX / 256;
+
 // the status of the launches so far, without leaving an error behind
 inline int launched() { return static_cast<int>(hipGetLastError()); }
 

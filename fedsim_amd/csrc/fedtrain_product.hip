@@ -1036,7 +1036,7 @@ Choice choose(const Args& a) {
 // 12; two 12.1 and 11.9, four 15.4 and 11.9; four f32 rows 20 and 25.  784 x 200:
 // 4 to 5 us, in place of 8 (bf16) and 11 (f32) by parts of k and their sum.
 bool few_rows(const Args& a) {
-  return a.form == FEDTRAIN_FORWARD && !a.groups && a.m <= 4 &&
+  return a.form == FEDTRAIN_FORWARD && !a.groups && a.m <= 4 && a.n < 1 << 28 &&
          (a.dtype == FEDTRAIN_F32 || a.m == 1 ||
           static_cast<double>(a.m) * a.n * a.k <= 1 << 24);
 }
@@ -1066,7 +1066,7 @@ template <int D, int FORM, class S> int go(const Args& a, int splits, hipStream_
   } else {
     all = p.tiles_m = a.groups ? a.m / S::BM + a.groups + 2 : (a.m + S::BM - 1) / S::BM;
   }
-  if (all > INT32_MAX / p.tiles_n) return FEDTRAIN_EINVAL;
+  if (all > kMostGroups / p.tiles_n) return FEDTRAIN_EINVAL;
   p.once = written_once<D>(a.m * a.n * (FORM == FEDTRAIN_GRAD_WEIGHT && a.groups ? a.groups : 1));
   // Bands of 4 (forward), 2 (grad input) and 8 rows (grad weight) took 1026, 1060
   // and 1122 us where 8, 8 and 4 took 1035, 1159 and 1151 (8192 x 4096 x 16384
@@ -1091,7 +1091,7 @@ template <int D, int FORM, class S> int go(const Args& a, int splits, hipStream_
   if (splits > 1) {
     if (const int rc = launched()) return rc;
     const int64_t eights = a.m * ((a.n + 7) / 8 + (a.colsum ? 1 : 0));
-    if (eights > static_cast<int64_t>(INT32_MAX) * 256) return FEDTRAIN_EINVAL;
+    if (eights > kMostGroups * 256) return FEDTRAIN_EINVAL;
     hipLaunchKernelGGL((k_join<D, FORM>), dim3(static_cast<unsigned>((eights + 255) / 256)),
                        dim3(256), 0, s, a, p);
   }
@@ -1161,7 +1161,7 @@ template <int D, int ACT> int slope(const Slope& given, hipStream_t s) {
     x.rows = 1;
   }
   const int64_t n = x.rows * ((x.cols + 7) / 8);
-  if (n > static_cast<int64_t>(INT32_MAX) * 256) return FEDTRAIN_EINVAL;
+  if (n > kMostGroups * 256) return FEDTRAIN_EINVAL;
   auto* kernel = written_once<D>(x.rows * x.cols) ? &k_act_backward<D, ACT, true>
                                                   : &k_act_backward<D, ACT, false>;
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, s,

@@ -47,7 +47,8 @@ extern "C" {
  * ascending row numbers on the device; rows offsets[g] .. offsets[g+1] use B
  * (FORWARD, GRAD_INPUT) or make C and colsum (GRAD_WEIGHT) at g * *_group.  A
  * row in no group gets C = res, or 0.  Offsets outside the rows are cut to
- * them: no value there makes an access leave the operands. */
+ * them: no value there makes an access leave the operands.
+ * More tiles than a launch can hold (2^24) are refused. */
 typedef struct fedtrain_product_args {
   int32_t dtype, form, act, groups;
   int64_t m, n, k;

@@ -496,3 +496,22 @@ def test_gradients_accumulate_and_a_changed_input_is_noticed():
         W.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         y.sum().backward()
+
+
+def test_negated_views_and_forward_mode():
+    """A tensor whose sign torch has put off is read with it; a forward-mode
+    derivative, which would be lost, raises."""
+    import torch.autograd.forward_ad as fwad
+
+    from fedsim_amd.functional import linear_act
+
+    gen = torch.Generator().manual_seed(21)
+    z = torch.randn(6, 5, generator=gen, dtype=torch.complex64).to(DEV)
+    x, w = z.conj().imag, _dev(_randn((4, 5), torch.float32, gen))
+    assert x.is_neg()
+    assert torch.equal(linear_act(x, w), linear_act(x.resolve_neg().contiguous(), w))
+    x = x.resolve_neg().contiguous()
+    with fwad.dual_level():
+        for a, b in ((fwad.make_dual(x, x), w), (x, fwad.make_dual(w, w))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                linear_act(a, b)

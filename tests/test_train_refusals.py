@@ -118,6 +118,17 @@ def test_plan_refusals(lib):
     assert lib.fedtrain_product_plan(None, r, r, r) == E
 
 
+def test_more_tiles_than_a_launch_holds(lib):
+    big = (1 << 31) - 1
+    for kw in (dict(m=big, n=1, k=1), dict(m=big, n=2, k=1, form=1, lda=1),
+               dict(m=big, n=2, k=1, form=2, ldc=4), dict(m=1, n=big, k=1, dtype=1, ldc=big)):
+        a = _args(**kw)
+        assert lib.fedtrain_product_workspace(ctypes.byref(a)) >= 0
+        assert lib.fedtrain_product(ctypes.byref(a), None) == E
+    assert lib.fedtrain_act_backward(1, 1, 1 << 18, 1 << 18, 64, 1 << 18, 64, 1 << 18, 64, 1 << 18,
+                                     None) == E
+
+
 def test_act_backward_refusals(lib):
     f = lib.fedtrain_act_backward
     ok = [0, 1, 2, 4, 64, 4, 64, 4, 64, 4, None]
@@ -253,6 +264,9 @@ def test_functions_refuse_what_does_not_fit():
                 lambda: train_ops.adamw_step([p], [p], [p], [p], step=1, lr=1e-3,
                                              betas=(0.9, 1.0)),
                 lambda: train_ops.adamw_step([p, p], [p, p], [p, p], [p, p], **ok),
+                lambda: train_ops.adamw_step([p[:200], p[100:]], [p[:200], p[100:]],
+                                             [t(200), t(200)], [t(200), t(200)], **ok),
+                lambda: train_ops.adamw_step([t(2), t(2)], [s, s], [s, s], [t(2), t(2)], **ok),
                 lambda: train_ops.adamw_step([p], [p], [p], [p], first_blocks=[], **ok)):
         with pytest.raises(ValueError):
             bad()
