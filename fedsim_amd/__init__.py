@@ -8,5 +8,13 @@ reference's names:
   fedsim_amd.utils.SerialAggregator                 (fedsim/utils/aggregators.py)
   fedsim_amd.distributed.centralized.training.FedAvg / AdaBest / FedNova
   fedsim_amd.distributed.centralized.CentralFLAlgorithm
+
+Beside it, operators for training the clients and the server's model on the GPU
+(libfedtrain.so, C-ABI in include/fedtrain.h):
+
+  fedsim_amd.functional   linear_act, grouped_linear: differentiable products
+                          with fused epilogues, of one model or a cohort
+  fedsim_amd.optim        AdamW in one launch, states in 32 or 8 bits
+  fedsim_amd.train_ops    the same without autograd
 """
 __version__ = "0.1.0"

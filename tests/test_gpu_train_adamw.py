@@ -179,6 +179,21 @@ def test_infinities_and_nan_are_that_elements_alone():
                                                  == float("inf")).all()
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_gradients_whose_squares_are_subnormal(bits):
+    """The first step is -lr sign(g) however small g is, with eps = 0.  v = 1e-2 g^2
+    of 1e-42 and more has 714 units of 2^-149 and is off by one: 0.0015, half of it
+    in the root."""
+    from fedsim_amd.optim import AdamW
+
+    g = torch.tensor([1e-20, -1e-20, 3e-20, 1e-19, -1e-17, 1e-12] * 100)
+    p = torch.nn.Parameter(torch.zeros(600, device=DEV))
+    p.grad = g.to(DEV)
+    AdamW([p], lr=0.5, betas=(0.9, 0.99), eps=0.0, weight_decay=0.0, state_bits=bits).step()
+    off = (p.detach().cpu() + 0.5 * torch.sign(g)).abs().max()
+    assert float(off) < 0.5 * (0.5 / 714 + 32 * 2.0 ** -24)
+
+
 def test_many_tensors_offsets_and_neighbours():
     """150 tensors of all alignments inside one buffer: more than a launch
     takes; what lies between them stays as it was."""
