@@ -20,7 +20,7 @@
 //                           3136 in 53 to 60 us with parts of k, 200 TFLOP/s at
 //                           larger sizes
 //   1000 clients' weights   memory: 3.5 GB of weights read once, 0.94 ms
-//   64 experts              tiles that ragged groups fill by two thirds: 590 to 710
+//   64 experts              tiles that ragged groups fill by two thirds: 520 to 710
 //                           us, of 400 by memory and 290 by the matrix unit
 //   a client's small batch  launches and the trip to memory: 5 to 9 us each
 #include "fedtrain_common.h"
@@ -413,9 +413,52 @@ template <int N> __device__ inline void wait_loads() {
 struct Plan {
   int64_t tiles_m, tiles_n;  // tiles_m: of one group (grad weight), or slots
   int high;                  // rows of tiles in a band, see place()
+  bool counted;              // see counted()
   bool once;                 // C is larger than what the caches could keep for a reader
   int splits;                // parts of k; over 1, C is f32 partial sums in the workspace
 };
+
+__device__ inline int tiles_of(const Args& a, int i, int BM) {
+  const int64_t n = bound(a, a.m, i + 1) - bound(a, a.m, i);
+  return n > 0 ? static_cast<int>((n + BM - 1) / BM) : 0;
+}
+
+// The rows and the column of tiles of a workgroup when every wave counts the
+// ranges' tiles, 64 ranges at a time, so that the dies share the tiles that exist
+// instead of the slots, of which ragged groups leave some empty.
+__device__ inline Rows counted(const Args& a, const Plan& plan, int BM, int64_t& tn) {
+  const int n = a.groups + 2, lane = threadIdx.x & 63;
+  const Rows none = {0, 0, -1};
+  int all = 0;
+  for (int i = lane; i < n; i += 64) all += tiles_of(a, i, BM);
+#pragma unroll
+  for (int s = 32; s; s >>= 1) all += __shfl_xor(all, s);
+  const int total = __builtin_amdgcn_readfirstlane(all);
+  if (static_cast<int64_t>(blockIdx.x) >= total * plan.tiles_n) return none;
+  int64_t slot;
+  place(total, plan.tiles_n, plan.high, slot, tn);
+  int before = 0;
+  for (int i0 = 0; i0 < n; i0 += 64) {
+    const int mine = i0 + lane < n ? tiles_of(a, i0 + lane, BM) : 0;
+    int upto = mine;
+#pragma unroll
+    for (int s = 1; s < 64; s *= 2) {
+      const int x = __shfl_up(upto, s);
+      if (lane >= s) upto += x;
+    }
+    const uint64_t over = __builtin_amdgcn_ballot_w64(before + upto > slot);
+    if (over) {
+      const int l = __builtin_ctzll(over), at = i0 + l;
+      const int64_t skipped = before + __builtin_amdgcn_readlane(upto - mine, l);
+      const int64_t first = bound(a, a.m, at), end = bound(a, a.m, at + 1);
+      const int64_t lo = first + (slot - skipped) * BM;
+      if (lo < first || lo >= end) return none;  // offsets that do not ascend
+      return {lo, lo + BM < end ? lo + BM : end, at - 1 < a.groups ? at - 1 : -1};
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  return none;
+}
 
 // ---------------------------------------------------------------------------
 // what becomes of the sums
@@ -539,8 +582,14 @@ void k_product(Args a, Plan plan) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / S::NW * (S::MI * 16), wn = wave % S::NW * (S::NI * 16);
-  int64_t slot, tn;
-  place(plan.tiles_m * (WEIGHT && a.groups ? a.groups : 1), plan.tiles_n, plan.high, slot, tn);
+  int64_t slot = 0, tn = 0;
+  Rows taken = {};
+  if (!WEIGHT && plan.counted) {
+    taken = counted(a, plan, S::BM, tn);
+  } else {
+    place(plan.tiles_m * (WEIGHT && a.groups ? a.groups : 1), plan.tiles_n, plan.high, slot, tn);
+    if (!WEIGHT) taken = rows_of(a, slot, S::BM);
+  }
   const int64_t col0 = tn * S::BN;
   int64_t row0, rows, k0 = 0, k1 = a.k;
   int group = 0;
@@ -554,11 +603,10 @@ void k_product(Args a, Plan plan) {
     row0 = slot * S::BM;
     rows = a.m - row0 < S::BM ? a.m - row0 : S::BM;
   } else {
-    const Rows r = rows_of(a, slot, S::BM);
-    if (r.lo >= r.hi) return;
-    row0 = r.lo;
-    rows = r.hi - r.lo;
-    group = r.group;
+    if (taken.lo >= taken.hi) return;
+    row0 = taken.lo;
+    rows = taken.hi - taken.lo;
+    group = taken.group;
     if (group < 0) k1 = 0;
   }
   if (plan.splits > 1) {  // an even part, in whole tiles
@@ -1105,6 +1153,11 @@ template <int D, int FORM, class S> int go(const Args& a, int splits, hipStream_
   // 695 and 1013 in bands of 8).
   p.high = FORM == FEDTRAIN_FORWARD ? 4 : FORM == FEDTRAIN_GRAD_INPUT ? 2 : 8;
   if (a.groups) p.high = FORM == FEDTRAIN_GRAD_WEIGHT ? 16 : 1;
+  // Counting pays up to two steps of 64 ranges and over four tiles a compute unit:
+  // grad input of 64 experts (2048 x 5632) 587 -> 521 us, 120 of f32 1024 x 1024 332
+  // -> 285, 126 of 1024 x 2048 159 -> 151; but 250 238 -> 247, 500 of 1024 x 1024 231
+  // -> 287, and ten small clients 17.6 -> 17.9.
+  p.counted = a.groups && a.groups <= 126 && all * p.tiles_n > 1024;
   constexpr int PLANES = D == FEDTRAIN_F32 ? 3 : 1;
   constexpr int STAGES = S::STAGES * PLANES * (S::BM + S::BN) * S::BK * 2 +
                          (D == FEDTRAIN_F32 ? 16 : 0);  // and the mark of an infinity

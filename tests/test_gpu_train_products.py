@@ -230,6 +230,22 @@ def test_grouped_widest_tiles(dtype, i, o):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("groups", [1, 62, 63, 126, 127])
+@pytest.mark.parametrize("i,o", [(40, 1104), (1101, 39)])
+def test_grouped_many_tiles(groups, i, o, dtype):
+    """More tiles than the card takes at a time, of as many ranges as are counted,
+    or one more: groups of very different sizes, a third of them empty, rows
+    before the first and behind the last."""
+    gen = torch.Generator().manual_seed(groups)
+    n = torch.exp(2 * torch.randn(groups, generator=gen)) * (torch.rand(groups, generator=gen) > .3)
+    n[0] += 0.1
+    edges = [3] + (3 + torch.round(n.cumsum(0) / n.sum() * 6990)).long().tolist()
+    N = 7000
+    x, w, b, r, dy = _case(N, i, o, dtype, 14, groups)
+    _check(x, w, b, r, dy, "silu", edges, torch.tensor(edges, device=DEV), on=DEV)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("residual", [False, True])
 def test_grouped_rows_of_no_group(dtype, residual):
     """Rows before the first and behind the last group: their residual or zero,
