@@ -561,8 +561,8 @@ template <int D, int FORM> struct Out {
 
 // A workgroup's tile of C.  16-bit operands whose chunks are whole and aligned go to
 // LDS directly (DIRECT): no registers and no instructions of the waves, which keeps
-// 256 sums a lane in registers of the largest tile and the matrix unit 75 % busy
-// (57 % with all of a stage's reads ahead of its products).  A tile of 256 x 256 by
+// 256 sums a lane in registers of the largest tile and the matrix unit busy for 75 %
+// of a steady run's cycles (57 % with a stage's reads ahead of its products).  A tile of 256 x 256 by
 // four waves reads 64 bytes of LDS for each product, half of what eight waves
 // would (30 % slower) and a quarter of what 128 x 128 by four does.  Operands at
 // any other alignment, and f32 on its way into three parts, come through

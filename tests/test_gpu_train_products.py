@@ -531,3 +531,45 @@ def test_negated_views_and_forward_mode():
         for a, b in ((fwad.make_dual(x, x), w), (x, fwad.make_dual(w, w))):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 linear_act(a, b)
+
+
+def test_two_at_once():
+    """Calls with workspaces (k in parts) on two streams at the same time, eager and
+    from two graphs: each has its own."""
+    from fedsim_amd.train_ops import product_forward, product_grad_weight
+
+    gen = torch.Generator().manual_seed(17)
+    sets = [(_randn((40, 5000), torch.bfloat16, gen).to(DEV),
+             _randn((96, 5000), torch.bfloat16, gen).to(DEV)) for _ in range(2)]
+
+    def run(x, w):
+        return [product_forward(x, w)[0],
+                product_grad_weight(x.t().contiguous(), w.t().contiguous())[0]]
+
+    want = [[t.cpu() for t in run(*s)] for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    graphs, kept = [], []
+    for s in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            kept.append(run(*s))
+        graphs.append(g)
+    torch.cuda.synchronize()
+    for _ in range(4):
+        got = []
+        for st, s in zip(streams, sets):
+            with torch.cuda.stream(st):
+                got.append([run(*s) for _ in range(4)][-1])
+        torch.cuda.synchronize()
+        for outs, w in zip(got, want):
+            assert all(torch.equal(a.cpu(), b) for a, b in zip(outs, w))
+        for outs in kept:
+            for t in outs:
+                t.zero_()
+        torch.cuda.synchronize()
+        for st, g in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for outs, w in zip(kept, want):
+            assert all(torch.equal(a.cpu(), b) for a, b in zip(outs, w))
