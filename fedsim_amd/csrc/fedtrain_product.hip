@@ -26,6 +26,7 @@
 #include "fedtrain_common.h"
 
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -76,7 +77,9 @@ template <int D, int ACT> __device__ inline float act_slope(float z) {
   }
   if constexpr (ACT == FEDTRAIN_ACT_SILU) {
     const float t = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -kLog2e));
-    return t * (1.0f + z * (1.0f - t));
+    // a finite sum may be an infinity in z's type: 0 and 1 there, not 0 times it
+    const float finite = fminf(fmaxf(z, -FLT_MAX), FLT_MAX);
+    return t * (1.0f + finite * (1.0f - t));
   }
   return 1.0f;
 }

@@ -1,0 +1,60 @@
+"""linear_act and act_backward where a type's range or a formula's cancellation
+decides: sums past float16, the far tails of the activations."""
+import pytest
+import torch
+
+import train_reference as R
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+DEV = "cuda"
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("act,below,above", [("none", 1, 1), ("relu", 0, 1), ("gelu", 0, 1),
+                                             ("silu", 0, 1)])
+def test_slopes_at_infinities(act, below, above, dtype):
+    """A z that its type holds as an infinity has the slope of the far ends; a
+    NaN has one of its own, or none."""
+    from fedsim_amd.train_ops import act_backward
+
+    inf = float("inf")
+    z = torch.tensor([[-inf, inf, -inf, inf, -1.0, 1.0, torch.finfo(dtype).min,
+                       torch.finfo(dtype).max]] * 3, dtype=dtype, device=DEV)
+    dy = torch.full_like(z, 3.0)
+    dz = act_backward(dy, z, act).cpu().double()
+    for k in (0, 2, 6):
+        assert (dz[:, k] == 3.0 * below).all(), (k, dz[0])
+    for k in (1, 3, 7):
+        assert (dz[:, k] == 3.0 * above).all(), (k, dz[0])
+
+
+@pytest.mark.parametrize("act", ["relu", "gelu", "silu"])
+@pytest.mark.parametrize("residual", [False, True])
+def test_float16_sums_past_its_range(act, residual):
+    """Sums of +-70400 and more in float16: act(-70400) is 0 and act(70400)
+    float16's infinity, with slopes of 0 and 1, so every gradient is finite and
+    exact.  Everything is a sum of few small whole numbers."""
+    from fedsim_amd.functional import linear_act
+
+    x = torch.zeros(8, 16, dtype=torch.float16)
+    x[:, 0] = torch.tensor([704., -704, 800, -800, 4, -1000, 1000, 0])
+    x[:, 1] = 1
+    w = torch.zeros(8, 16, dtype=torch.float16)
+    w[:, 0] = 100  # every row's sums are 100 x0: +-70400, +-80000, 400, +-100000, 0
+    dy = torch.ones(8, 8, dtype=torch.float16)
+    dy[:, 3] = 2
+    r = torch.full((8, 8), 5.0, dtype=torch.float16) if residual else None
+    X, W = x.to(DEV).requires_grad_(True), w.to(DEV).requires_grad_(True)
+    B = torch.zeros(8, dtype=torch.float16, device=DEV, requires_grad=True)
+    y = linear_act(X, W, B, None if r is None else r.to(DEV), activation=act)
+    z = 100.0 * x[:, :1].double().expand(8, 8)
+    want = R.act(z, act) + (5.0 if residual else 0.0)
+    assert torch.equal(y.detach().cpu(), want.to(torch.float16))
+    dx, dw, db = torch.autograd.grad(y, (X, W, B), dy.to(DEV))
+    slope = R.slope(z, act)
+    dz = dy.double() * slope
+    assert torch.equal(dx.cpu().double(), (dz @ w.double()))
+    assert torch.equal(dw.cpu().double(), (dz.T @ x.double()))
+    assert torch.equal(db.cpu().double(), dz.sum(0))
