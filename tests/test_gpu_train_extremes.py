@@ -1,5 +1,7 @@
 """linear_act and act_backward where a type's range or a formula's cancellation
 decides: sums past float16, the far tails of the activations."""
+import math
+
 import pytest
 import torch
 
@@ -58,3 +60,35 @@ def test_float16_sums_past_its_range(act, residual):
     assert torch.equal(dx.cpu().double(), (dz @ w.double()))
     assert torch.equal(dw.cpu().double(), (dz.T @ x.double()))
     assert torch.equal(db.cpu().double(), dz.sum(0))
+
+
+def _tail_error(z):
+    """How far Phi(z) and z phi(z) in float32 may be off, relative: 13 units of
+    2^-24 for the approximation, 24 for its terms' roundings and the hardware's
+    reciprocal and exponential, and z^2 / 2, the exponent, off by 4.5 units of its
+    own; a library's erfc takes 32 and an argument rounded once."""
+    return (40 + 4 * z * z) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_gelus_tail(dtype):
+    """gelu(z) = z Phi(z) and its slope are good relative to themselves for
+    negative z too, where 1 + erf(z / sqrt 2) cancels."""
+    from fedsim_amd.functional import linear_act
+    from fedsim_amd.train_ops import act_backward
+
+    low = {torch.float32: -12.5, torch.bfloat16: -12.5, torch.float16: -6.0}[dtype]
+    z = torch.linspace(low, 6.0, 20_011, dtype=torch.float64).to(dtype)
+    y = linear_act(z[:, None].to(DEV), torch.ones(1, 1, dtype=dtype, device=DEV),
+                   activation="gelu")
+    z = z.double()
+    cdf = torch.erfc(z * -math.sqrt(0.5)) / 2  # torch's ndtr cancels below -8
+    far = z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    want = z * cdf
+    e = _tail_error(z) * want.abs()
+    R.close(y[:, 0], (want, e + R.HALF[dtype] * (want.abs() + e) + R.TINY[dtype]), "gelu")
+    dz = act_backward(torch.ones(1, z.numel(), dtype=dtype, device=DEV),
+                      z.to(dtype)[None].to(DEV), "gelu")
+    want = cdf + far
+    e = _tail_error(z) * (cdf + far.abs())
+    R.close(dz[0], (want, e + R.HALF[dtype] * (want.abs() + e) + R.TINY[dtype]), "slope")
