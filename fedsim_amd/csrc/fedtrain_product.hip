@@ -164,11 +164,15 @@ __device__ inline int group_of(const Args& a, int64_t row) {
 // with the transposing load.  In both a line's chunks are exchanged by xor, so
 // that the lanes that LDS serves together meet different banks.
 //
-// f32 operands are split into three bf16 parts by cutting off bits, x = h + m + l
-// exactly, one plane each; the six products hh, hm, mh, hl, mm, lh keep all but
-// 2^-21 of |a b| (after Henry, Tang and Heinecke, 2019: the bf16 unit is 16
-// times the f32 unit's rate, so six products are 2.7 times faster than one).
+// f32 operands are split into three bf16 parts, x = h + m + l exactly, each the
+// nearest to what is left, one plane each.  With 2^e <= |x| < 2^(e+1), |m| <=
+// 2^(e-8) and |l| <= 2^(e-17), so the six products hh, hm, mh, hl, mm, lh keep all
+// but 2^-24 of |a b|, one rounding of an f32 product (cutting bits off instead
+// would leave out up to 2^-21, always towards zero).  After Henry, Tang and
+// Heinecke, 2019: the bf16 unit is 16 times the f32 unit's rate, so six products
+// are 2.7 times faster than one.
 
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(4))) short s16x4;
@@ -217,19 +221,35 @@ template <bool KS_, int W_, int BK_> struct Tile {
   }
 };
 
-// x's three bf16 parts, in the high halves, with garbage below them.  True for an
-// infinity or NaN, whose parts are wrong.  (Parts below 2^-126 may be lost.)
-__device__ inline bool split3(float x, unsigned& h, unsigned& m, unsigned& l) {
+// The parts of two neighbouring values, packed as they lie in LDS.  True for an
+// infinity or NaN, or a number that rounds to an infinity, whose parts are wrong.
+// (Parts below 2^-126 may be lost.)
+__device__ inline bool split3(f32x2 x, unsigned* to) {
+  auto up = [](unsigned two) {
+    return f32x2{__builtin_bit_cast(float, two << 16),
+                 __builtin_bit_cast(float, two & 0xFFFF0000u)};
+  };
+  f32x2 r = x;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    to[i] = __builtin_bit_cast(unsigned, __builtin_convertvector(r, bf16x2));
+    if (i < 2) {
+      const f32x2 part = up(to[i]);
+      r[0] -= part[0];
+      r[1] -= part[1];
+    }
+  }
+  return r[0] != r[0] || r[1] != r[1];
+}
+
+// The same for any value, by cutting off bits: an infinity or NaN is its first
+// part alone.
+__device__ inline void split3_any(float x, unsigned& h, unsigned& m, unsigned& l) {
   h = __builtin_bit_cast(unsigned, x);
   const float r = x - __builtin_bit_cast(float, h & 0xFFFF0000u);
   m = __builtin_bit_cast(unsigned, r);
   l = __builtin_bit_cast(unsigned, r - __builtin_bit_cast(float, m & 0xFFFF0000u));
-  return r != r;
-}
-
-// The same with an infinity or NaN as its first part alone.
-__device__ inline void split3_any(float x, unsigned& h, unsigned& m, unsigned& l) {
-  if (!split3(x, h, m, l)) return;
+  if (r == r) return;
   m = l = 0;
   if (x != x) h |= 0x10000u;  // a NaN stays one
 }
@@ -351,8 +371,8 @@ template <int D, class L, int THREADS, bool DIRECT> struct Loader {
     }
   }
 
-  // chunk i to its place; f32: true where an infinity or NaN was met, whose parts
-  // are right with ANY alone
+  // chunk i to its place; f32: true where a value was met whose parts are right with
+  // ANY alone
   template <bool ANY> __device__ bool put(int i, char* to, int tid) const {
     char* p = to + (tid + i * THREADS) * 16;
     bool met = false;
@@ -362,18 +382,20 @@ template <int D, class L, int THREADS, bool DIRECT> struct Loader {
       u32x4 out[3];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        unsigned h[2], m[2], l[2];
+        const f32x4 four = __builtin_bit_cast(f32x4, held[i][e / 2]);
+        const f32x2 x = {four[e % 2 * 2], four[e % 2 * 2 + 1]};
+        unsigned part[3];
+        if constexpr (ANY) {
+          unsigned b[2][3];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const int n = e * 2 + s;
-          const unsigned bits = held[i][n / 4][n % 4];
-          const float x = __builtin_bit_cast(float, bits);
-          if (ANY) split3_any(x, h[s], m[s], l[s]);
-          else met |= split3(x, h[s], m[s], l[s]);
+          for (int s = 0; s < 2; ++s) split3_any(x[s], b[s][0], b[s][1], b[s][2]);
+#pragma unroll
+          for (int j = 0; j < 3; ++j) part[j] = __builtin_amdgcn_perm(b[1][j], b[0][j], 0x07060302);
+        } else {
+          met |= split3(x, part);
         }
-        out[0][e] = __builtin_amdgcn_perm(h[1], h[0], 0x07060302);
-        out[1][e] = __builtin_amdgcn_perm(m[1], m[0], 0x07060302);
-        out[2][e] = __builtin_amdgcn_perm(l[1], l[0], 0x07060302);
+#pragma unroll
+        for (int j = 0; j < 3; ++j) out[j][e] = part[j];
       }
 #pragma unroll
       for (int e = 0; e < 3; ++e) *reinterpret_cast<u32x4*>(p + e * L::bytes) = out[e];
@@ -742,7 +764,7 @@ void k_product(Args a, Plan plan) {
       if (tid == 0) *odd = 0;
       __syncthreads();
     }
-    // the loaded tile to LDS; an infinity or NaN leaves its mark
+    // the loaded tile to LDS; a value that ANY is for leaves its mark
     auto fill = [&](char* to) {
       bool met = la.template put_all<false>(to, tid);
       met |= lb.template put_all<false>(to + PLANES * LA::bytes, tid);

@@ -92,3 +92,41 @@ def test_gelus_tail(dtype):
     want = cdf + far
     e = _tail_error(z) * (cdf + far.abs())
     R.close(dz[0], (want, e + R.HALF[dtype] * (want.abs() + e) + R.TINY[dtype]), "slope")
+
+
+def test_float32_products_of_few_terms():
+    """float32 products in three bf16 parts, for sums too short to hide what is
+    left out: 2^-24 of each product, (1 + 2^-9) of it.  A sum of K takes 2^-23
+    for each addition where the matrix unit cuts off, and the smaller parts' own
+    sums, at most 2^-6 of it in four instructions, 2^-27."""
+    from fedsim_amd.functional import linear_act
+    from fedsim_amd.train_ops import product_grad_weight
+
+    gen = torch.Generator().manual_seed(31)
+    for K in (1, 2, 3):
+        x = torch.randn(K, 700, generator=gen)
+        d = torch.randn(K, 300, generator=gen)
+        dw, _ = product_grad_weight(d.to(DEV), x.to(DEV))
+        S = d.double().abs().T @ x.double().abs()
+        e = (2.0 ** -24 + 2.0 ** -23 * K + 2.0 ** -26) * S
+        R.close(dw, (d.double().T @ x.double(), e), f"dw {K}")
+        a, b = x.T.contiguous(), d.T.contiguous()
+        y = linear_act(a.to(DEV), b.to(DEV))
+        R.close(y, (a.double() @ b.double().T, e.T), f"y {K}")
+
+
+@pytest.mark.parametrize("tiny", [2.0 ** -100, 2.0 ** -112, 2.0 ** -120, 2.0 ** -126, 2.0 ** -135])
+def test_float32_factors_next_to_the_smallest(tiny):
+    """A factor's bf16 parts below 2^-126 may be lost: two of them at most, the
+    larger below 2^-126 and the other 2^-8 of it, so a factor is off by 2^-125
+    at most, next to the rounding of normal sums."""
+    from fedsim_amd.functional import linear_act
+
+    gen = torch.Generator().manual_seed(32)
+    x = torch.randn(40, 64, generator=gen).double() * tiny
+    x = x.to(torch.float32)  # subnormals for the last two
+    w = torch.randn(24, 64, generator=gen)
+    y = linear_act(x.to(DEV), w.to(DEV))
+    S = x.double().abs() @ w.double().abs().T
+    e = R.sum_error(64, S) + 2.0 ** -125 * w.double().abs().sum(1)[None] + 64 * R.TINY[torch.float32]
+    R.close(y, (x.double() @ w.double().T, e.expand(40, 24)), str(tiny))
