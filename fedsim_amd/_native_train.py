@@ -18,7 +18,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libfedtrain.so")
 
 # Must match include/fedtrain.h
-ABI_VERSION = 1
+ABI_VERSION = 2
 FEDTRAIN_EINVAL = -22
 FEDTRAIN_F32, FEDTRAIN_BF16, FEDTRAIN_F16 = 0, 1, 2
 FEDTRAIN_ACT_NONE, FEDTRAIN_ACT_RELU, FEDTRAIN_ACT_GELU, FEDTRAIN_ACT_SILU = 0, 1, 2, 3
@@ -48,7 +48,7 @@ class AdamWScalars(ctypes.Structure):
     _fields_ = ([(n, ctypes.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay")]
                 + [("step", ctypes.c_int64), ("seed", ctypes.c_uint32),
                    ("maximize", ctypes.c_int32), ("device_step", ctypes.c_void_p),
-                   ("workspace", ctypes.c_void_p)])
+                   ("workspace", ctypes.c_void_p), ("device_steps", ctypes.c_void_p)])
 
 
 # struct fedtrain_adamw_tensor as eight 64-bit words: p, g, m, v, m_scale,

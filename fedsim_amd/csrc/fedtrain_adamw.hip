@@ -48,7 +48,8 @@ struct Batch {
   int count;
   float b1, c1, b2, c2, decay, eps, size, root;
   unsigned key;
-  const float* device;  // {size, root, key} computed on the device, or null
+  const float* device;  // {size, root, key} computed on the device, or null:
+  int each;             // floats from one tensor's to the next one's, 0 if they share them
 };
 
 // two rounds of xor-shift and multiply by odd fractions of sqrt(2) and sqrt(3)
@@ -296,7 +297,10 @@ template <int D, int BITS, int PER> __global__ __launch_bounds__(256) void k_ada
   const Tensor& t = b.at[i];
   const int64_t chunk = static_cast<int64_t>(blockIdx.x - t.first) * (PER * 1024);
   Scalars c = {b.size, b.root, b.key};
-  if (b.device) c = {b.device[0], b.device[1], to_bits(b.device[2])};
+  if (b.device) {
+    const float* d = b.device + i * b.each;
+    c = {d[0], d[1], to_bits(d[2])};
+  }
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if (PER == 4 && t.wide() && chunk + PER * 1024 <= t.n()) {
     if constexpr (BITS == 8) {
@@ -326,9 +330,15 @@ __host__ __device__ inline Corrections corrections(double lr, double b1, double 
           static_cast<float>(1 / sqrt(1 - pow(b2, t)))};
 }
 
-__global__ void k_adamw_scalars(double lr, double b1, double b2, unsigned seed,
-                                const int64_t* step, float* out) {
-  const int64_t t = *step;
+struct Steps {
+  const int64_t* at[kMost];
+};
+
+// A thread for each count on the device.
+__global__ void k_adamw_scalars(double lr, double b1, double b2, unsigned seed, Steps steps,
+                                float* out) {
+  const int64_t t = *steps.at[threadIdx.x];
+  out += threadIdx.x * 4;
   const Corrections c = corrections(lr, b1, b2, static_cast<double>(t));
   out[0] = c.size;
   out[1] = c.root;
@@ -355,7 +365,7 @@ extern "C" int fedtrain_adamw(int dtype, int state_bits, int64_t count,
   if (dtype < FEDTRAIN_F32 || dtype > FEDTRAIN_F16 || (state_bits != 8 && state_bits != 32) ||
       count < 0 || (count && !tensors) || !s)
     return FEDTRAIN_EINVAL;
-  if (s->device_step ? !s->workspace || !aligned(s->workspace, 4) : s->step < 1)
+  if (s->device_step || s->device_steps ? !s->workspace || !aligned(s->workspace, 4) : s->step < 1)
     return FEDTRAIN_EINVAL;
   if (!(s->beta1 >= 0 && s->beta1 < 1 && s->beta2 >= 0 && s->beta2 < 1 && s->lr >= 0 &&
         s->eps >= 0 && s->weight_decay >= 0))
@@ -373,6 +383,8 @@ extern "C" int fedtrain_adamw(int dtype, int state_bits, int64_t count,
         (!t.m_scale || !t.v_scale || !aligned(t.m_scale, 4) || !aligned(t.v_scale, 4)))
       return FEDTRAIN_EINVAL;
     if (t.n > kMostGroups * 1024) return FEDTRAIN_EINVAL;
+    if (s->device_steps && !(s->device_steps[i] && aligned(s->device_steps[i], 8)))
+      return FEDTRAIN_EINVAL;
     total += t.n;
   }
   // below 4 workgroups of 1024 elements a compute unit the smaller ones win
@@ -386,12 +398,22 @@ extern "C" int fedtrain_adamw(int dtype, int state_bits, int64_t count,
   b.decay = static_cast<float>(1 - s->lr * s->weight_decay);
   b.eps = static_cast<float>(s->eps);
   b.device = nullptr;
+  b.each = 0;
   b.size = b.root = 0;
   b.key = 0;
-  if (s->device_step) {
-    b.device = static_cast<const float*>(s->workspace);
-    hipLaunchKernelGGL(k_adamw_scalars, dim3(1), dim3(1), 0, st, s->lr, s->beta1, s->beta2,
-                       s->seed, s->device_step, static_cast<float*>(s->workspace));
+  Steps steps;
+  float* scalars = static_cast<float*>(s->workspace);  // of the launch's first tensor
+  auto count_on_device = [&](int n) {
+    b.device = scalars;
+    hipLaunchKernelGGL(k_adamw_scalars, dim3(1), dim3(n), 0, st, s->lr, s->beta1, s->beta2,
+                       s->seed, steps, scalars);
+    return launched();
+  };
+  if (s->device_steps) {
+    b.each = 4;
+  } else if (s->device_step) {
+    steps.at[0] = s->device_step;
+    if (const int rc = count_on_device(1)) return rc;
   } else {
     const Corrections c = corrections(s->lr, s->beta1, s->beta2, static_cast<double>(s->step));
     b.size = c.size;
@@ -406,6 +428,7 @@ extern "C" int fedtrain_adamw(int dtype, int state_bits, int64_t count,
       if (!t.n) continue;
       const int64_t groups = (t.n + per * 1024 - 1) / (per * 1024);
       if (grid + groups > kMostGroups) break;
+      if (s->device_steps) steps.at[b.count] = s->device_steps[i];
       Tensor& at = b.at[b.count++];
       at.p = t.p;
       at.g = t.g;
@@ -420,6 +443,10 @@ extern "C" int fedtrain_adamw(int dtype, int state_bits, int64_t count,
       grid += groups;
     }
     if (!b.count) break;
+    if (s->device_steps) {
+      if (const int rc = count_on_device(b.count)) return rc;
+      scalars += 4 * b.count;
+    }
     const unsigned n = static_cast<unsigned>(grid);
     if (dtype == FEDTRAIN_F32) launch<FEDTRAIN_F32>(state_bits, per, n, st, b);
     else if (dtype == FEDTRAIN_BF16) launch<FEDTRAIN_BF16>(state_bits, per, n, st, b);

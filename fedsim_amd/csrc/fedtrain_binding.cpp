@@ -410,7 +410,8 @@ void apart(const Tensors& ts, const char* name) {
 void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& ms,
                 const Tensors& vs, const optional<Tensors>& m_scales,
                 const optional<Tensors>& v_scales, int64_t step,
-                const optional<Tensor>& device_step, double lr, double b1, double b2, double eps,
+                const optional<Tensor>& device_step, const optional<Tensors>& device_steps,
+                double lr, double b1, double b2, double eps,
                 double weight_decay, bool maximize, int64_t seed,
                 const optional<std::vector<int64_t>>& first_blocks) {
   TORCH_CHECK_VALUE(lr >= 0 && b1 >= 0 && b1 < 1 && b2 >= 0 && b2 < 1 && eps >= 0 &&
@@ -471,13 +472,26 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& ms,
   s.maximize = maximize;
   const On at(d);
   Tensor work;
-  if (device_step) {
-    TORCH_CHECK_VALUE(device_step->scalar_type() == at::kLong && device_step->device() == d &&
-                          device_step->numel() == 1,
+  std::vector<const int64_t*> counts;
+  auto count_of = [&](const Tensor& t) {
+    TORCH_CHECK_VALUE(t.scalar_type() == at::kLong && t.device() == d && t.numel() == 1,
                       "a step on the device must be one int64 on ", d);
-    work = at::empty({4}, at::TensorOptions().dtype(at::kFloat).device(d));
-    s.device_step = static_cast<const int64_t*>(device_step->const_data_ptr());
+    return static_cast<const int64_t*>(t.const_data_ptr());
+  };
+  auto scratch = [&](size_t tensors) {
+    work = at::empty({static_cast<int64_t>(4 * tensors)},
+                     at::TensorOptions().dtype(at::kFloat).device(d));
     s.workspace = work.mutable_data_ptr();
+  };
+  if (device_steps) {
+    TORCH_CHECK_VALUE(device_steps->size() == n, "steps: ", device_steps->size(),
+                      " counts for ", n, " parameters");
+    for (const Tensor& t : *device_steps) counts.push_back(count_of(t));
+    s.device_steps = counts.data();
+    scratch(n);
+  } else if (device_step) {
+    s.device_step = count_of(*device_step);
+    scratch(1);
   } else {
     TORCH_CHECK_VALUE(step >= 1, "steps are counted from 1, got ", step);
     s.step = step;

@@ -22,11 +22,11 @@ class AdamW(torch.optim.Optimizer):
     two for each 256 elements: 2 bytes an element instead of 8.  The codes are
     rounded stochastically from ``seed``, the step's number and the element's.
 
-    ``capturable=True`` counts the steps on the device, together for the
-    parameters of a group, so that a captured graph of ``step()`` goes on
-    counting when it is replayed; capture after the first eager step, which
-    makes the states.  Otherwise each parameter counts its own steps on the host
-    and a capture raises.
+    Each parameter counts its own steps, as a parameter without a gradient sits a
+    step out: on the host, or with ``capturable=True`` on the device, so that a
+    captured graph of ``step()`` goes on counting when it is replayed.  Capture
+    after an eager step, which makes the states; without ``capturable`` a capture
+    raises.
 
     Parameters are contiguous float32, bfloat16 or float16 tensors; a 16-bit
     parameter is rounded to nearest each step.  The step of a captured graph
@@ -82,6 +82,12 @@ class AdamW(torch.optim.Optimizer):
                                            "the states")
                     self._init_state(p, group, st)
                 if group["capturable"]:
+                    if not isinstance(st["step"], torch.Tensor):
+                        if capturing:  # a replay would start again
+                            raise RuntimeError("take a step before capturing one: the first "
+                                               "puts the count on the device")
+                        st["step"] = torch.full((1,), int(st["step"]), dtype=torch.int64,
+                                                device=p.device)
                     key = (p.dtype, p.device, None)
                 elif capturing:
                     raise RuntimeError("AdamW counts its steps on the host: a captured graph "
@@ -90,14 +96,10 @@ class AdamW(torch.optim.Optimizer):
                     st["step"] = int(st["step"]) + 1
                     key = (p.dtype, p.device, st["step"])
                 todo.setdefault(key, []).append((p, st, first))
-            counted = {}
-            for (_, dev, n), items in todo.items():
+            for (_, _, n), items in todo.items():
                 if n is None:
-                    n = counted.get(dev)
-                    if n is None:
-                        n = counted[dev] = self._count(group, dev)
-                    for _, st, _ in items:
-                        st["step"] = n
+                    n = [st["step"] for _, st, _ in items]
+                    torch._foreach_add_(n, 1)
                 eight = group["state_bits"] == 8
                 train_ops.adamw_step(
                     [p for p, _, _ in items], [p.grad.contiguous() for p, _, _ in items],
@@ -109,25 +111,6 @@ class AdamW(torch.optim.Optimizer):
                     weight_decay=group["weight_decay"], maximize=group["maximize"],
                     seed=group["seed"], first_blocks=[f for _, _, f in items])
         return loss
-
-    def _count(self, group, dev) -> torch.Tensor:
-        """The group's step on ``dev``, one further: the tensor that every
-        parameter's state holds."""
-        n = None
-        for p in group["params"]:
-            st = self.state.get(p)
-            if st and p.device == dev and isinstance(st["step"], torch.Tensor):
-                n = st["step"]
-                break
-        if n is None:
-            if torch.cuda.is_current_stream_capturing():  # a replay would start again
-                raise RuntimeError("take a step before capturing one: the first puts the count "
-                                   "on the device")
-            known = [int(self.state[p]["step"]) for p in group["params"] if self.state.get(p)
-                     and p.device == dev]
-            n = torch.full((1,), max(known, default=0), dtype=torch.int64, device=dev)
-        n.add_(1)
-        return n
 
     def load_state_dict(self, state_dict):
         """torch's, with the states in their own types: torch would cast them

@@ -87,9 +87,12 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     ``first_blocks[i]`` where given), so a step is the same each time it is run.
 
     ``step``: 1 for the first step; or an int64 tensor of one element on the
-    device, read when the step runs (for a captured graph)."""
-    device_step = step if isinstance(step, torch.Tensor) else None
+    device, read when the step runs (for a captured graph), or one such tensor
+    for each parameter."""
+    one = step if isinstance(step, torch.Tensor) else None
+    each = step if isinstance(step, (list, tuple)) else None
     _native_train.ext().adamw_step(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales,
-                                   exp_avg_sq_scales, 0 if device_step is not None else int(step),
-                                   device_step, lr, betas[0], betas[1], eps, weight_decay,
-                                   maximize, seed, first_blocks)
+                                   exp_avg_sq_scales,
+                                   int(step) if one is None and each is None else 0, one, each,
+                                   lr, betas[0], betas[1], eps, weight_decay, maximize, seed,
+                                   first_blocks)

@@ -21,7 +21,7 @@
 extern "C" {
 #endif
 
-#define FEDTRAIN_ABI_VERSION 1
+#define FEDTRAIN_ABI_VERSION 2
 #define FEDTRAIN_EINVAL (-22)
 
 #define FEDTRAIN_F32 0
@@ -107,11 +107,14 @@ typedef struct fedtrain_adamw_tensor {
 
 typedef struct fedtrain_adamw_scalars {
   double lr, beta1, beta2, eps, weight_decay;
-  int64_t step; /* 1 for the first; not read when device_step is given */
+  int64_t step; /* 1 for the first; not read when a step on the device is given */
   uint32_t seed;
   int32_t maximize;
   const int64_t* device_step; /* the step's number on the device, or NULL */
-  void* workspace;            /* 16 bytes on the device, with device_step */
+  void* workspace;            /* 16 bytes on the device with device_step, 16 for each
+                                 tensor with device_steps */
+  const int64_t* const* device_steps; /* on the host: where on the device each tensor's
+                                         own step is, or NULL (then device_step is not read) */
 } fedtrain_adamw_scalars;
 
 int fedtrain_adamw(int dtype, int state_bits, int64_t count, const fedtrain_adamw_tensor* tensors,
