@@ -12,6 +12,7 @@
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <string>
 #include <tuple>
 #include <vector>
@@ -393,18 +394,38 @@ void same(const Tensors& ts, const char* name, at::ScalarType type, const at::De
   }
 }
 
-// Two workgroups would write the same elements.
-void apart(const Tensors& ts, const char* name) {
-  std::vector<std::pair<uintptr_t, uintptr_t>> at;
-  at.reserve(ts.size());
-  for (const Tensor& t : ts) {
-    const auto p = reinterpret_cast<uintptr_t>(t.const_data_ptr());
-    if (t.numel()) at.emplace_back(p, p + t.nbytes());
+struct Listed {
+  const Tensors& tensors;
+  const char* name;
+  bool written;
+};
+
+// What is written shares memory with nothing else: two workgroups would write the
+// same elements, or one read what another has already changed.
+void apart(std::initializer_list<Listed> lists) {
+  struct Range {
+    uintptr_t begin, end;
+    const Listed* of;
+  };
+  std::vector<Range> at;
+  at.reserve(lists.size() * lists.begin()->tensors.size());
+  for (const Listed& list : lists)
+    for (const Tensor& t : list.tensors) {
+      const auto p = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+      if (t.numel()) at.push_back({p, p + t.nbytes(), &list});
+    }
+  std::sort(at.begin(), at.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
+  // the ranges that reach furthest so far: of those written, and of the others
+  const Range none = {0, 0, nullptr};
+  Range written = none, read = none;
+  for (const Range& r : at) {
+    for (const Range* other : {&written, &read})
+      TORCH_CHECK_VALUE(r.begin >= other->end || !(r.of->written || other->of->written),
+                        other->of->name, " and ", r.of->name,
+                        " share memory: a tensor is given once");
+    Range& far = r.of->written ? written : read;
+    if (r.end > far.end) far = r;
   }
-  std::sort(at.begin(), at.end());
-  for (size_t i = 1; i < at.size(); ++i)
-    TORCH_CHECK_VALUE(at[i].first >= at[i - 1].second, "two of ", name,
-                      " share memory: a tensor is given once");
 }
 
 void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& ms,
@@ -439,13 +460,13 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& ms,
     same(*m_scales, "exp_avg_scales", at::kFloat, d, blocks);
     same(*v_scales, "exp_avg_sq_scales", at::kFloat, d, blocks);
   }
-  apart(params, "params");
-  apart(ms, "exp_avgs");
-  apart(vs, "exp_avg_sqs");
-  if (eight) {
-    apart(*m_scales, "exp_avg_scales");
-    apart(*v_scales, "exp_avg_sq_scales");
-  }
+  const Tensors no_scales;
+  apart({{params, "params", true},
+         {grads, "grads", false},
+         {ms, "exp_avgs", true},
+         {vs, "exp_avg_sqs", true},
+         {eight ? *m_scales : no_scales, "exp_avg_scales", true},
+         {eight ? *v_scales : no_scales, "exp_avg_sq_scales", true}});
   TORCH_CHECK_VALUE(!first_blocks || first_blocks->size() == n, "first_blocks: one for each of ",
                     n, " parameters");
   std::vector<fedtrain_adamw_tensor> table(n);

@@ -93,7 +93,8 @@ int fedtrain_act_backward(int dtype, int act, int64_t rows, int64_t cols, const 
 /* One tensor of an AdamW step: n elements; g has p's type; m and v are f32
  * (state_bits 32), or e4m3 and e5m2 codes with one f32 scale for each 256
  * elements in m_scale and v_scale (state_bits 8).  block0 numbers the tensor's
- * first block of 256 in the whole step, for the rounding's random numbers. */
+ * first block of 256 in the whole step, for the rounding's random numbers.  What a
+ * step writes (p, m, v, the scales) shares memory with nothing else it is given. */
 typedef struct fedtrain_adamw_tensor {
   void* p;
   const void* g;

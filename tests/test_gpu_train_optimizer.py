@@ -153,3 +153,53 @@ def test_many_counted_steps_on_the_device():
                  [one] * 129 + [one.expand(2)], [one] * 129 + [1]):
         with pytest.raises((ValueError, TypeError)):
             adamw_step(*bad, step=step, lr=1e-2)
+
+
+def test_what_a_step_writes_shares_no_memory():
+    """Each list against each other one; gradients may share among themselves."""
+    from fedsim_amd.train_ops import adamw_step
+
+    f8, f8v = torch.float8_e4m3fn, torch.float8_e5m2
+
+    def f32(n=300):
+        return torch.ones(n, device=DEV)
+
+    hy = dict(step=1, lr=1e-3)
+    p = f32()
+    two = f32(600)
+    for bad in ([p, p, f32(), f32()], [p, f32(), p, f32()], [p, f32(), f32(), p],
+                [f32(), p, p, f32()], [f32(), p, f32(), p], [f32(), f32(), p, p],
+                [two[:300], two[200:500], f32(), f32()],  # a gradient at an offset
+                [two[200:500], two[:300], f32(), f32()],
+                [two[:300], f32(), two[299:599], f32()],
+                [f32(), f32(), two[299:599], two[:300]]):
+        with pytest.raises(ValueError, match="share memory"):
+            adamw_step(*[[t] for t in bad], **hy)
+
+    def eight():
+        return [f32(), f32(), f32().to(f8), f32().to(f8v), f32(2), f32(2)]
+
+    one = eight()
+    raw = torch.zeros(600, dtype=torch.uint8, device=DEV)
+    for k, t in ((5, one[4]), (4, one[0][:2]), (5, one[0][298:]), (5, one[1][:2]),
+                 (2, raw[:300].view(f8)), (2, one[0].view(torch.uint8)[:300].view(f8))):
+        bad = list(one)
+        bad[k] = t
+        if t.dtype == f8 and t.data_ptr() == raw.data_ptr():
+            bad[3] = raw[100:400].view(f8v)
+        with pytest.raises(ValueError, match="share memory"):
+            adamw_step(*[[t] for t in bad], **hy)
+    # a long range behind which short ones lie: the furthest counts
+    slab = f32(1000)
+    with pytest.raises(ValueError, match="share memory"):
+        adamw_step([slab[:900], slab[950:]], [f32(900), f32(50)], [f32(900), f32(50)],
+                   [f32(900), slab[800:850]], **hy)
+    assert (two == 1).all() and (slab == 1).all() and (p == 1).all()
+    g = f32(600)
+    a, b = f32(), f32()
+    adamw_step([a, b], [g[:300], g[100:400]], [torch.zeros_like(a) for _ in range(2)],
+               [torch.zeros_like(a) for _ in range(2)], **hy)
+    assert torch.equal(a, b) and (a < 1).all()
+    # neighbours in one buffer share nothing
+    slab = torch.rand(1200, device=DEV)
+    adamw_step(*[[slab[k * 300:(k + 1) * 300]] for k in range(4)], **hy)
