@@ -8,7 +8,11 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <torch/csrc/jit/frontend/tracer.h>
+
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
@@ -29,6 +33,20 @@ constexpr int64_t kStateBlock = 256;
 
 void check(int status, const char* what) {
   TORCH_CHECK(status == 0, what, " failed (", status, "): ", fedtrain_strerror(status));
+}
+
+// A tracer sees torch's own operators alone: of a call here the allocation of its
+// results, which a replay would return as they come.
+void not_traced() {
+  using Mode = c10::impl::TorchDispatchModeKey;
+  bool traced = torch::jit::tracer::isTracing() ||
+                c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch);
+  if (c10::impl::TorchDispatchModeTLS::any_modes_set())
+    for (const Mode m : {Mode::FAKE, Mode::PROXY, Mode::FUNCTIONAL})
+      traced |= c10::impl::TorchDispatchModeTLS::get_mode(m).has_value();
+  TORCH_CHECK_NOT_IMPLEMENTED(!traced, "the training operators cannot be traced (torch.jit.trace, "
+                                       "make_fx, torch.export): a graph would hold their "
+                                       "results' allocation alone");
 }
 
 int dtype_of(const Tensor& t, const char* name) {
@@ -129,6 +147,7 @@ Tensor make(at::IntArrayRef sizes, const Tensor& like) {
 std::tuple<Tensor, Tensor> forward_of(const Tensor& x_, const Tensor& w_,
                                       const optional<Tensor>& b_, const optional<Tensor>& r_,
                                       int act, const optional<Tensor>& offsets, bool want_z) {
+  not_traced();
   require(x_, "x");
   require(w_, "weight", x_);
   const bool grouped = offsets.has_value();
@@ -183,6 +202,7 @@ std::tuple<Tensor, Tensor> forward_of(const Tensor& x_, const Tensor& w_,
 }
 
 Tensor grad_input_of(const Tensor& dz_, const Tensor& w_, const optional<Tensor>& offsets) {
+  not_traced();
   require(dz_, "dz");
   require(w_, "weight", dz_);
   const bool grouped = offsets.has_value();
@@ -216,6 +236,7 @@ Tensor grad_input_of(const Tensor& dz_, const Tensor& w_, const optional<Tensor>
 std::tuple<Tensor, Tensor> grad_weight_of(const Tensor& dz_, const Tensor& x_,
                                           const optional<Tensor>& offsets, bool want_weight,
                                           bool want_bias) {
+  not_traced();
   require(x_, "x");
   require(dz_, "dz", x_);
   TORCH_CHECK_VALUE(dz_.dim() == 2 && x_.dim() == 2 && dz_.size(0) == x_.size(0), "dz ",
@@ -254,6 +275,7 @@ std::tuple<Tensor, Tensor> grad_weight_of(const Tensor& dz_, const Tensor& x_,
 }
 
 Tensor act_backward_of(const Tensor& dy_, const Tensor& z_, int act) {
+  not_traced();
   require(dy_, "dy");
   require(z_, "z", dy_);
   TORCH_CHECK_VALUE(dy_.dim() == 2 && dy_.sizes() == z_.sizes(), "dy ", dy_.sizes(), " and z ",
@@ -349,6 +371,7 @@ Tensor product(const Tensor& x, const Tensor& w, const optional<Tensor>& b,
 
 Tensor linear_act(const Tensor& x, const Tensor& w, const optional<Tensor>& b,
                   const optional<Tensor>& r, const std::string& activation) {
+  not_traced();
   const int act = activation_of(activation);
   require(x, "x");
   require(w, "weight", x);
@@ -435,6 +458,7 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& ms,
                 double lr, double b1, double b2, double eps,
                 double weight_decay, bool maximize, int64_t seed,
                 const optional<std::vector<int64_t>>& first_blocks) {
+  not_traced();
   TORCH_CHECK_VALUE(lr >= 0 && b1 >= 0 && b1 < 1 && b2 >= 0 && b2 < 1 && eps >= 0 &&
                         weight_decay >= 0,
                     "lr ", lr, ", betas (", b1, ", ", b2, "), eps ", eps, ", weight_decay ",

@@ -12,7 +12,8 @@ The value before the activation is kept for the gradient in the tensors' type.
 
 A backward pass may be captured into a graph together with its forward pass;
 as with any torch operator, no eager graph of the same leaves may be alive then.
-They can be differentiated once.
+They can be differentiated once, and cannot be traced (torch.jit.trace, make_fx,
+torch.export); torch.compile calls them between its graphs.
 """
 from __future__ import annotations
 

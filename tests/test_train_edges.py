@@ -28,3 +28,74 @@ def test_counts_on_the_device_are_checked():
     for kw in (dict(steps=(64, 0)), dict(steps=(0, 64)), dict(steps=(64, 68)),
                dict(steps=(64, 64), workspace=None), dict(steps=(64, 64), workspace=66)):
         assert call(**kw) == E, kw
+
+
+def _calls():
+    """(name, function of two tensors, its arguments' shapes)."""
+    from fedsim_amd import train_ops
+    from fedsim_amd.functional import grouped_linear, linear_act
+
+    off = torch.tensor([0, 3])
+    return [
+        ("linear_act", lambda x, w: linear_act(x, w), (3, 4), (5, 4)),
+        ("grouped_linear", lambda x, w: grouped_linear(x, w[None], off), (3, 4), (5, 4)),
+        ("forward", lambda x, w: train_ops.product_forward(x, w)[0], (3, 4), (5, 4)),
+        ("grad_input", lambda d, w: train_ops.product_grad_input(d, w), (3, 5), (5, 4)),
+        ("grad_weight", lambda d, x: train_ops.product_grad_weight(d, x)[0], (3, 5), (3, 4)),
+        ("act_backward", lambda d, z: train_ops.act_backward(d, z, "relu"), (3, 5), (3, 5)),
+        ("adamw_step", lambda p, g: train_ops.adamw_step(
+            [p], [g], [g * 0], [g * 0], step=1, lr=1e-3), (8,), (8,)),
+    ]
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("k", range(7))
+def test_tracing_is_refused(k):
+    """A recorded graph would hold the allocation of the results and not what
+    fills them."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    name, f, a, b = _calls()[k]
+    x, y = torch.randn(a), torch.randn(b)
+
+    class Module(torch.nn.Module):
+        def forward(self, x, y):
+            return f(x, y)
+
+    def fake():
+        with FakeTensorMode():
+            f(torch.empty(a, device="cuda"), torch.empty(b, device="cuda"))
+
+    for trace in (lambda: torch.jit.trace(f, (x, y)), lambda: make_fx(f)(x, y),
+                  lambda: make_fx(f, tracing_mode="fake")(x, y),
+                  lambda: make_fx(f, tracing_mode="symbolic")(x, y),
+                  lambda: make_fx(f, pre_dispatch=True)(x, y),
+                  lambda: torch.export.export(Module(), (x, y), strict=False), fake):
+        with pytest.raises(NotImplementedError, match="traced"):
+            trace()
+    with pytest.raises(ValueError, match="HIP device"):  # and nothing of it stays behind
+        f(x, y)
+
+
+@pytest.mark.gpu
+@pytest.mark.filterwarnings("ignore")
+def test_transforms_raise_and_compile_breaks_its_graph():
+    """torch.func's wrapped tensors have no memory to read; torch.compile calls
+    the operators outside its graphs."""
+    from torch.utils.flop_counter import FlopCounterMode
+
+    from fedsim_amd.functional import linear_act
+
+    gen = torch.Generator().manual_seed(1)
+    x, w = torch.randn(3, 4, generator=gen).cuda(), torch.randn(5, 4, generator=gen).cuda()
+    for bad in (lambda: torch.vmap(lambda a: linear_act(a, w))(torch.stack([x, x])),
+                lambda: torch.func.grad(lambda a: linear_act(a, w).sum())(x),
+                lambda: torch.func.functionalize(lambda a: linear_act(a, w))(x)):
+        with pytest.raises(RuntimeError):
+            bad()
+    want = linear_act(x, w, activation="gelu")
+    got = torch.compile(lambda a: linear_act(a * 1, w, activation="gelu") * 1, backend="eager")(x)
+    assert torch.equal(got, want)
+    with FlopCounterMode(display=False):  # a mode that looks on is no tracer
+        assert torch.equal(linear_act(x, w, activation="gelu"), want)
