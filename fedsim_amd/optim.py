@@ -93,23 +93,32 @@ class AdamW(torch.optim.Optimizer):
                     raise RuntimeError("AdamW counts its steps on the host: a captured graph "
                                        "needs capturable=True")
                 else:
-                    st["step"] = int(st["step"]) + 1
-                    key = (p.dtype, p.device, st["step"])
+                    key = (p.dtype, p.device, int(st["step"]) + 1)
                 todo.setdefault(key, []).append((p, st, first))
             for (_, _, n), items in todo.items():
+                counts = None
                 if n is None:
-                    n = [st["step"] for _, st, _ in items]
-                    torch._foreach_add_(n, 1)
+                    counts = [st["step"] for _, st, _ in items]
+                    torch._foreach_add_(counts, 1)
                 eight = group["state_bits"] == 8
-                train_ops.adamw_step(
-                    [p for p, _, _ in items], [p.grad.contiguous() for p, _, _ in items],
-                    [st["exp_avg"] for _, st, _ in items],
-                    [st["exp_avg_sq"] for _, st, _ in items],
-                    [st["exp_avg_scale"] for _, st, _ in items] if eight else None,
-                    [st["exp_avg_sq_scale"] for _, st, _ in items] if eight else None,
-                    step=n, lr=float(group["lr"]), betas=group["betas"], eps=group["eps"],
-                    weight_decay=group["weight_decay"], maximize=group["maximize"],
-                    seed=group["seed"], first_blocks=[f for _, _, f in items])
+                try:
+                    train_ops.adamw_step(
+                        [p for p, _, _ in items], [p.grad.contiguous() for p, _, _ in items],
+                        [st["exp_avg"] for _, st, _ in items],
+                        [st["exp_avg_sq"] for _, st, _ in items],
+                        [st["exp_avg_scale"] for _, st, _ in items] if eight else None,
+                        [st["exp_avg_sq_scale"] for _, st, _ in items] if eight else None,
+                        step=n if counts is None else counts, lr=float(group["lr"]),
+                        betas=group["betas"], eps=group["eps"],
+                        weight_decay=group["weight_decay"], maximize=group["maximize"],
+                        seed=group["seed"], first_blocks=[f for _, _, f in items])
+                except Exception:  # a step that was not taken is not counted
+                    if counts is not None:
+                        torch._foreach_sub_(counts, 1)
+                    raise
+                if counts is None:
+                    for _, st, _ in items:
+                        st["step"] = n
         return loss
 
     def load_state_dict(self, state_dict):

@@ -155,6 +155,27 @@ def test_many_counted_steps_on_the_device():
             adamw_step(*bad, step=step, lr=1e-2)
 
 
+@pytest.mark.parametrize("capturable", [False, True])
+def test_a_step_that_raises_is_not_counted(capturable):
+    """A gradient of another size than its parameter's (a parameter resized
+    through .data), mended: the next step is the second."""
+    gen, a, b, ours, theirs = _pair([64, 10], 6, capturable=capturable)
+    _grads(gen, a, b)
+    ours.step()
+    theirs.step()
+    _grads(gen, a, b)
+    whole = a[1].data
+    a[1].data = torch.zeros(11, device=DEV)
+    with pytest.raises(ValueError):
+        ours.step()
+    a[1].data = whole
+    assert [int(ours.state[p]["step"]) for p in a] == [1, 1]
+    ours.step()
+    theirs.step()
+    assert [int(ours.state[p]["step"]) for p in a] == [2, 2]
+    _same(a, b, 2)
+
+
 def test_what_a_step_writes_shares_no_memory():
     """Each list against each other one; gradients may share among themselves."""
     from fedsim_amd.train_ops import adamw_step
