@@ -396,7 +396,9 @@ extern "C" int fedtrain_adamw(int dtype, int state_bits, int64_t count,
   b.b2 = static_cast<float>(s->beta2);
   b.c2 = static_cast<float>(1 - s->beta2);
   b.decay = static_cast<float>(1 - s->lr * s->weight_decay);
-  b.eps = static_cast<float>(s->eps);
+  // below the smallest normal number its reciprocal would be an infinity, and m = 0
+  // times it NaN; the root of any v above 0 is far larger
+  b.eps = s->eps > 0 ? fmaxf(static_cast<float>(s->eps), 0x1p-126f) : 0.0f;
   b.device = nullptr;
   b.each = 0;
   b.size = b.root = 0;

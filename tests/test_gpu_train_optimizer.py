@@ -176,6 +176,20 @@ def test_a_step_that_raises_is_not_counted(capturable):
     _same(a, b, 2)
 
 
+def test_an_epsilon_below_the_smallest_normal_number():
+    """m = 0 and v = 0 over eps: no change, for every eps above 0."""
+    from fedsim_amd.train_ops import adamw_step
+
+    for eps in (1e-30, 1e-39, 1e-45, 1e-60):
+        p, g = torch.full((300,), 2.0, device=DEV), torch.zeros(300, device=DEV)
+        g[7] = 1.0
+        m, v = torch.zeros(300, device=DEV), torch.zeros(300, device=DEV)
+        adamw_step([p], [g], [m], [v], step=1, lr=0.5, eps=eps, weight_decay=0.0)
+        assert abs(float(p[7]) - 1.5) < 32 * 2.0 ** -24
+        p[7] = 2.0
+        assert (p == 2.0).all(), eps
+
+
 def test_what_a_step_writes_shares_no_memory():
     """Each list against each other one; gradients may share among themselves."""
     from fedsim_amd.train_ops import adamw_step
