@@ -124,9 +124,24 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """torch's, with the states in their own types: torch would cast them
         to the parameters'.  As there, the groups' options are the saved ones,
-        ``state_bits`` among them."""
+        ``state_bits`` among them; those that a state of torch.optim.AdamW lacks
+        stay as they are."""
+        saved = state_dict["param_groups"]
+        lacking = [{k: v for k, v in mine.items() if k not in g}
+                   for mine, g in zip(self.param_groups, saved)]
+        for mine, g in zip(lacking, saved):
+            for name, only in (("amsgrad", False), ("decoupled_weight_decay", True)):
+                if g.get(name, only) != only:
+                    raise ValueError(f"AdamW has no {name}={g[name]}")
+            bits = g.get("state_bits", mine.get("state_bits"))
+            for i in g["params"]:
+                held = state_dict["state"].get(i, {}).get("exp_avg")
+                if held is not None and held.dtype != _STATES[bits][0]:
+                    raise ValueError(f"a {held.dtype} exp_avg does not fit state_bits={bits}")
         super().load_state_dict(state_dict)
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for g, mine in zip(self.param_groups, lacking):
+            g.update(mine)
+        ids = [i for g in saved for i in g["params"]]
         ps = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(ids, ps):
             given = state_dict["state"].get(i)

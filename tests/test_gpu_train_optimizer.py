@@ -190,6 +190,39 @@ def test_an_epsilon_below_the_smallest_normal_number():
         assert (p == 2.0).all(), eps
 
 
+def test_a_state_of_torchs_adamw():
+    """Its options lack this class's own, which stay as they were given; what
+    this class does not have is refused."""
+    from fedsim_amd.optim import AdamW
+
+    gen = torch.Generator().manual_seed(8)
+    b = [torch.nn.Parameter(torch.randn(n, generator=gen)) for n in (100, 33)]
+    theirs = torch.optim.AdamW(b, lr=1e-2, weight_decay=0.1)
+    for _ in range(3):
+        for q in b:
+            q.grad = torch.randn(q.shape, generator=gen)
+        theirs.step()
+    two = [torch.nn.Parameter(q.detach().to(DEV)) for q in b]
+    opt = AdamW(two, seed=5)
+    opt.load_state_dict(theirs.state_dict())
+    assert opt.param_groups[0]["state_bits"] == 32 and opt.param_groups[0]["seed"] == 5
+    for p, q in zip(two, b):
+        q.grad = torch.randn(q.shape, generator=gen)
+        p.grad = q.grad.to(DEV)
+    opt.step()
+    theirs.step()
+    assert [int(opt.state[p]["step"]) for p in two] == [4, 4]
+    for p, q in zip(two, b):  # a step each in float32
+        q = q.detach().double()
+        R.close(p, (q, 2 * 24 * 2.0 ** -24 * (q.abs() + 0.3)), "p")
+    with pytest.raises(ValueError, match="state_bits"):
+        AdamW(two, state_bits=8).load_state_dict(theirs.state_dict())
+    saved = torch.optim.AdamW(b, amsgrad=True).state_dict()
+    with pytest.raises(ValueError, match="amsgrad"):
+        opt.load_state_dict(saved)
+    assert not opt.param_groups[0].get("amsgrad")
+
+
 def test_what_a_step_writes_shares_no_memory():
     """Each list against each other one; gradients may share among themselves."""
     from fedsim_amd.train_ops import adamw_step
