@@ -299,7 +299,8 @@ template <int D, class L, int THREADS, bool DIRECT> struct Loader {
   // apart, would wait for all of them before the next LDS read: arrive() and
   // wait_loads() are what orders them.  They have no result in a register.  A
   // descriptor's registers may come from the vector unit, 5 cycles before a load
-  // may read them.
+  // may read them.  m0 cannot be named as changed, it is the compiler's own: a test
+  // reads the listing for any other use of it.
   __device__ u32x4 descriptor(int64_t k) const {
     const uint64_t p = reinterpret_cast<uint64_t>(base + (L::KS ? k * ld : k));
     u32x4 d;

@@ -1,9 +1,13 @@
 """The training operators' edges that need no device: C arguments, tracing, what
 the compiler spilled."""
 import ctypes
+import re
+import subprocess
 
 import pytest
 import torch
+
+from test_train_isa import NM, _instructions, objects  # noqa: F401  (one a fixture)
 
 E = -22
 
@@ -99,3 +103,37 @@ def test_transforms_raise_and_compile_breaks_its_graph():
     assert torch.equal(got, want)
     with FlopCounterMode(display=False):  # a mode that looks on is no tracer
         assert torch.equal(linear_act(x, w, activation="gelu"), want)
+
+
+def test_m0_belongs_to_the_direct_loads(objects):
+    """The loads to LDS set m0 in assembly, and the compiler takes no such clobber
+    (m0 is reserved): so nothing it emits may name m0 itself, or read it unnamed."""
+    sets = loads = 0
+    for co in objects:
+        last = []
+        for _, op, args in _instructions(co):
+            if "m0" in args.replace(",", " ").split():
+                assert op == "s_mov_b32" and args.startswith("m0, s"), (op, args)
+                sets += 1
+            # what reads m0 without naming it
+            assert not op.startswith(("v_movrel", "s_movrel", "s_set_gpr_idx", "v_interp",
+                                      "s_sendmsg", "ds_gws", "s_ttracedata")), op
+            if " lds" in args or op.startswith("global_load_lds"):
+                loads += 1
+                assert op.startswith("buffer_load") and [o for o, _ in last[-2:]] == \
+                    ["s_mov_b32", "s_nop"] and last[-2][1].startswith("m0"), last
+            last = (last + [(op, args)])[-2:]
+    assert sets == loads > 1000
+
+
+def test_spilled_registers(objects):
+    """No vector register is spilled; of scalars the widest grad weight keeps five in a
+    vector register's lanes."""
+    seen = 0
+    for co in objects:
+        notes = subprocess.check_output([NM, "--notes", co], text=True)
+        for key, most in ((".vgpr_spill_count", 0), (".sgpr_spill_count", 8)):
+            counts = [int(n) for n in re.findall(re.escape(key) + r":\s+(\d+)", notes)]
+            assert counts and max(counts) <= most, (key, counts)
+            seen += len(counts)
+    assert seen > 100
