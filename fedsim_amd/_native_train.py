@@ -51,10 +51,6 @@ class AdamWScalars(ctypes.Structure):
                    ("workspace", ctypes.c_void_p), ("device_steps", ctypes.c_void_p)])
 
 
-# struct fedtrain_adamw_tensor as eight 64-bit words: p, g, m, v, m_scale,
-# v_scale, n, block0
-ADAMW_WORDS = 8
-
 SIGNATURES = {
     "fedtrain_abi_version": (ctypes.c_int, []),
     "fedtrain_strerror": (ctypes.c_char_p, [ctypes.c_int]),

@@ -11,7 +11,6 @@ namespace fedtrain {
 typedef __attribute__((ext_vector_type(2))) float f32x2;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
-typedef __attribute__((ext_vector_type(2))) unsigned u32x2;
 
 // 16-bit types convert from f32 to the nearest value, ties to even
 template <int D> struct Elem;

@@ -177,7 +177,6 @@ typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 typedef __attribute__((ext_vector_type(8))) short s16x8;
-typedef __attribute__((address_space(3))) char lds_char;
 
 template <int D> __device__ inline f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
   if constexpr (D == FEDTRAIN_F16)
