@@ -18,7 +18,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libfedtrain.so")
 
 # Must match include/fedtrain.h
-ABI_VERSION = 2
+ABI_VERSION = 3
 FEDTRAIN_EINVAL = -22
 FEDTRAIN_F32, FEDTRAIN_BF16, FEDTRAIN_F16 = 0, 1, 2
 FEDTRAIN_ACT_NONE, FEDTRAIN_ACT_RELU, FEDTRAIN_ACT_GELU, FEDTRAIN_ACT_SILU = 0, 1, 2, 3
@@ -39,6 +39,19 @@ class ProductArgs(ctypes.Structure):
                    ("colsum", ctypes.c_void_p), ("colsum_group", ctypes.c_int64),
                    ("offsets", ctypes.c_void_p), ("offsets64", ctypes.c_int32),
                    ("reserved", ctypes.c_int32),
+                   ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64)])
+
+
+class ActArgs(ctypes.Structure):
+    """struct fedtrain_act_args (include/fedtrain.h)."""
+
+    _fields_ = ([(n, ctypes.c_int32) for n in ("dtype", "act", "groups", "offsets64")]
+                + [("rows", ctypes.c_int64), ("cols", ctypes.c_int64),
+                   ("dy", ctypes.c_void_p), ("lddy", ctypes.c_int64),
+                   ("z", ctypes.c_void_p), ("ldz", ctypes.c_int64),
+                   ("dz", ctypes.c_void_p), ("lddz", ctypes.c_int64),
+                   ("colsum", ctypes.c_void_p), ("colsum_group", ctypes.c_int64),
+                   ("offsets", ctypes.c_void_p),
                    ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64)])
 
 
@@ -66,6 +79,8 @@ SIGNATURES = {
          ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,
          ctypes.c_void_p],
     ),
+    "fedtrain_act_backward_sums_workspace": (ctypes.c_int64, [ctypes.POINTER(ActArgs)]),
+    "fedtrain_act_backward_sums": (ctypes.c_int, [ctypes.POINTER(ActArgs), ctypes.c_void_p]),
     "fedtrain_adamw": (
         ctypes.c_int,
         [ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.c_void_p,

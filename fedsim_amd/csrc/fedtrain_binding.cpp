@@ -108,8 +108,8 @@ struct On {
   void* stream;
 };
 
-int groups_of(int64_t groups, const Tensor& offsets, const at::Device& d,
-              fedtrain_product_args* a) {
+template <class Args>
+int groups_of(int64_t groups, const Tensor& offsets, const at::Device& d, Args* a) {
   TORCH_CHECK_TYPE(offsets.scalar_type() == at::kInt || offsets.scalar_type() == at::kLong,
                    "offsets must be int32 or int64, got ", offsets.scalar_type());
   TORCH_CHECK_VALUE(offsets.device() == d, "offsets must live on ", d, ", got ",
@@ -292,6 +292,48 @@ Tensor act_backward_of(const Tensor& dy_, const Tensor& z_, int act) {
   return dz;
 }
 
+// (dz, db) of a 16-bit dy: db from the terms before they are rounded.
+std::tuple<Tensor, Tensor> act_backward_sums_of(const Tensor& dy_, const Tensor& z_, int act,
+                                                const optional<Tensor>& offsets) {
+  not_traced();
+  require(dy_, "dy");
+  require(z_, "z", dy_);
+  TORCH_CHECK_VALUE(dy_.dim() == 2 && dy_.sizes() == z_.sizes(), "dy ", dy_.sizes(), " and z ",
+                    z_.sizes(), " must be one [N, out]");
+  fits(dy_.size(0), "rows");
+  fits(dy_.size(1), "outputs");
+  const Tensor dy = rows(dy_), z = rows(z_);
+  fedtrain_act_args a = {};
+  a.dtype = dtype_of(dy, "dy");
+  a.act = act;
+  if (offsets) groups_of(-1, *offsets, dy.device(), &a);
+  const int64_t M = dy.size(1);
+  Tensor dz = make(dy.sizes(), dy);
+  Tensor db = offsets ? make({a.groups, M}, dy) : make({M}, dy);
+  a.rows = dy.size(0);
+  a.cols = M;
+  a.dy = dy.const_data_ptr();
+  a.lddy = step(dy);
+  a.z = z.const_data_ptr();
+  a.ldz = step(z);
+  a.dz = dz.mutable_data_ptr();
+  a.lddz = M;
+  a.colsum = db.mutable_data_ptr();
+  a.colsum_group = M;
+  const On at(dy.device());
+  Tensor work;
+  const int64_t need = fedtrain_act_backward_sums_workspace(&a);
+  TORCH_CHECK(need >= 0, "fedtrain_act_backward_sums_workspace failed (", need,
+              "): ", fedtrain_strerror(static_cast<int>(need)));
+  if (need > 0) {
+    work = at::empty({need}, dy.options().dtype(at::kByte).requires_grad(false));
+    a.workspace = work.mutable_data_ptr();
+    a.workspace_bytes = need;
+  }
+  check(fedtrain_act_backward_sums(&a, at.stream), "fedtrain_act_backward_sums");
+  return {dz, db};
+}
+
 // ---------------------------------------------------------------------------
 // the differentiable product
 // ---------------------------------------------------------------------------
@@ -338,9 +380,20 @@ struct Product : torch::autograd::Function<Product> {
       const at::NoGradGuard no_grad;
       if (dy.defined() && (nx || nw || nb)) {
         const int act = static_cast<int>(ctx->saved_data["act"].toInt());
-        const Tensor dz = kept.defined() ? act_backward_of(dy, kept, act) : dy;
+        Tensor dz = dy;
+        if (kept.defined()) {
+          if (nb && dy.scalar_type() != at::kFloat)
+            std::tie(dz, db) = act_backward_sums_of(dy, kept, act, offsets);
+          else
+            dz = act_backward_of(dy, kept, act);
+        }
         if (nx) dx = grad_input_of(dz, w, offsets);
-        if (nw || nb) std::tie(dw, db) = grad_weight_of(dz, nw ? x : dz, offsets, nw, nb);
+        const bool sum = nb && !db.defined();
+        if (nw || sum) {
+          auto [weight, bias] = grad_weight_of(dz, nw ? x : dz, offsets, nw, sum);
+          dw = weight;
+          if (sum) db = bias;
+        }
       }
     }
     torch::autograd::variable_list out = {dx, dw, db, nr ? dy : Tensor(), Tensor(), Tensor()};

@@ -7,7 +7,12 @@
 //   grad weight   C = A^T B, colsum = A^T 1                A = dz, B = x
 //
 // Sums, bias, activation and residual are f32; C and z are rounded to their type
-// once, at the store.  The activation's gradient is taken at the rounded z.
+// once, at the store.  The activation's gradient is taken at the rounded z, and
+// dz = dy act'(z) is rounded to the type before dx and dW, whose matrix instructions
+// take operands of that type: in 16 bits they are 0.0024 (bf16) and 0.0003 (f16) from
+// the exact result in the mean, where their own rounding alone makes 0.0017 and
+// 0.0002.  f32 z and dz would be twice the bytes, and dz in two parts twice the
+// products.  db is summed from dz as it is before that.
 //
 // One kernel (k_product) in tiles of 256 x 256, 128 x 128 and 64 x 64 (f32: 64 x
 // 128), picked by choose().  What bounds it, as measured on one MI355X (a copy
@@ -1029,6 +1034,74 @@ __global__ __launch_bounds__(256) void k_act_backward(int64_t rows, int64_t cols
   write8<D, ONCE>(static_cast<T*>(dz) + r * lddz + c, n, g);
 }
 
+// The same where a bias wants its gradient too, in 16-bit types: its terms are added
+// up before they are rounded (rounded ones put db off 1.5 times as far as its own
+// rounding does, by several of its units where the terms cancel).  A workgroup takes
+// 64 columns of up to kSumRows rows of a group, 8 values a thread and 128 rows at a
+// time; sums go through the wave, LDS and, where there is more than one such part,
+// the workspace, in the same order in every run.
+constexpr int kSumRows = 2048, kSumCols = 64;
+
+template <int D, int ACT, bool ONCE>
+__global__ __launch_bounds__(1024) void k_act_backward_sums(Args a, int64_t strips, bool joined) {
+  using T = typename Elem<D>::type;
+  __shared__ float part[16][kSumCols];
+  const int64_t slot = blockIdx.x / strips, col0 = blockIdx.x % strips * kSumCols;
+  const Rows taken = rows_of(a, slot, kSumRows);
+  if (joined && taken.lo >= taken.hi) return;
+  const int lane = threadIdx.x & 63, c = (threadIdx.x & 7) * 8;
+  const int64_t col = col0 + c;
+  const int n = static_cast<int>(a.n - col < 8 ? a.n - col : 8);
+  float sum[8] = {};
+  if (n > 0) {
+#pragma unroll 2
+    for (int64_t r = taken.lo + (threadIdx.x >> 3); r < taken.hi; r += 128) {
+      float g[8], x[8];
+      read8<D>(a.a, r * a.lda + col, n, g);
+      read8<D>(a.b, r * a.ldb + col, n, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        g[e] *= act_slope<D, ACT>(x[e]);
+        sum[e] += g[e];
+      }
+      write8<D, ONCE>(static_cast<T*>(a.c) + r * a.ldc + col, n, g);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+#pragma unroll
+    for (int s = 8; s < 64; s *= 2) sum[e] += __shfl_xor(sum[e], s);
+    if (lane < 8) part[threadIdx.x >> 6][c + e] = sum[e];
+  }
+  __syncthreads();
+  if (threadIdx.x >= kSumCols || col0 + threadIdx.x >= a.n) return;
+  float all = 0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) all += part[w][threadIdx.x];
+  if (joined) static_cast<float*>(a.workspace)[slot * a.n + col0 + threadIdx.x] = all;
+  else static_cast<T*>(a.colsum)[col0 + threadIdx.x] = Elem<D>::down(all);
+}
+
+// A group's parts, a thread for each of its columns.
+template <int D> __global__ __launch_bounds__(256) void k_sums_join(Args a) {
+  using T = typename Elem<D>::type;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (id >= (a.groups ? a.groups : 1) * a.n) return;
+  const int64_t group = id / a.n, col = id % a.n;
+  int64_t lo = 0, hi = a.m, slot = 0;
+  if (a.groups) {  // as rows_of() deals them out
+    const int i = static_cast<int>(group) + 1;
+    lo = bound(a, a.m, i);
+    hi = bound(a, a.m, i + 1);
+    slot = lo / kSumRows + i;
+  }
+  float all = 0;
+#pragma unroll 4
+  for (; lo < hi; lo += kSumRows, ++slot)
+    all += static_cast<const float*>(a.workspace)[slot * a.n + col];
+  static_cast<T*>(a.colsum)[group * a.colsum_group + col] = Elem<D>::down(all);
+}
+
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
@@ -1291,6 +1364,75 @@ template <int D> int slope(int act, const Slope& x, hipStream_t s) {
   return slope<D, FEDTRAIN_ACT_NONE>(x, s);
 }
 
+bool valid(const fedtrain_act_args* x) {
+  if (!x || (x->dtype != FEDTRAIN_BF16 && x->dtype != FEDTRAIN_F16) || x->act < FEDTRAIN_ACT_NONE ||
+      x->act > FEDTRAIN_ACT_SILU || x->groups < 0 || x->groups > INT32_MAX - 2 || x->rows < 0 ||
+      x->cols < 0 || x->rows > kMaxSize || x->cols > kMaxSize)
+    return false;
+  if (x->groups && (!x->offsets || !aligned(x->offsets, x->offsets64 ? 8 : 4))) return false;
+  const void* each[] = {x->dy, x->z, x->dz, x->colsum};
+  for (const void* p : each)
+    if (!aligned(p, 2)) return false;
+  if (x->lddy < 0 || x->ldz < 0 || (x->rows > 1 && x->lddz < x->cols) ||
+      (x->groups > 1 && x->colsum_group < x->cols))
+    return false;
+  return !x->cols || (x->colsum && (!x->rows || (x->dy && x->z && x->dz)));
+}
+
+// Parts of rows, and whether their sums have to be joined: not where one workgroup
+// sees all rows of its columns.
+int64_t sum_slots(const fedtrain_act_args& x) {
+  if (x.groups) return x.rows / kSumRows + x.groups + 2;
+  return std::max<int64_t>(1, (x.rows + kSumRows - 1) / kSumRows);
+}
+bool sums_joined(const fedtrain_act_args& x) { return x.groups || x.rows > kSumRows; }
+
+int64_t workspace(const fedtrain_act_args& x) {
+  return sums_joined(x) ? sum_slots(x) * x.cols * 4 : 0;
+}
+
+template <int D, int ACT> int slope_sums(const fedtrain_act_args& x, hipStream_t s) {
+  const int64_t strips = (x.cols + kSumCols - 1) / kSumCols, slots = sum_slots(x);
+  const int64_t sums = (x.groups ? x.groups : 1) * x.cols;
+  const bool joined = sums_joined(x);
+  // a launch's threads are counted in 32 bits
+  if (slots > UINT32_MAX / 1024 / strips || sums > kMostGroups * 256) return FEDTRAIN_EINVAL;
+  if (joined && (!x.workspace || !aligned(x.workspace, 16) || x.workspace_bytes < workspace(x)))
+    return FEDTRAIN_EINVAL;
+  Args a = {};
+  a.groups = x.groups;
+  a.offsets = x.offsets;
+  a.offsets64 = x.offsets64;
+  a.m = x.rows;
+  a.n = x.cols;
+  a.a = x.dy;
+  a.lda = x.lddy;
+  a.b = x.z;
+  a.ldb = x.ldz;
+  a.c = x.dz;
+  a.ldc = x.lddz;
+  a.colsum = x.colsum;
+  a.colsum_group = x.colsum_group;
+  a.workspace = x.workspace;
+  auto* kernel = written_once<D>(x.rows * x.cols) ? &k_act_backward_sums<D, ACT, true>
+                                                  : &k_act_backward_sums<D, ACT, false>;
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(slots * strips)), dim3(1024), 0, s, a,
+                     strips, joined);
+  if (joined) {
+    if (const int rc = launched()) return rc;
+    hipLaunchKernelGGL((k_sums_join<D>), dim3(static_cast<unsigned>((sums + 255) / 256)),
+                       dim3(256), 0, s, a);
+  }
+  return launched();
+}
+
+template <int D> int slope_sums(const fedtrain_act_args& x, hipStream_t s) {
+  if (x.act == FEDTRAIN_ACT_RELU) return slope_sums<D, FEDTRAIN_ACT_RELU>(x, s);
+  if (x.act == FEDTRAIN_ACT_GELU) return slope_sums<D, FEDTRAIN_ACT_GELU>(x, s);
+  if (x.act == FEDTRAIN_ACT_SILU) return slope_sums<D, FEDTRAIN_ACT_SILU>(x, s);
+  return slope_sums<D, FEDTRAIN_ACT_NONE>(x, s);
+}
+
 }  // namespace
 
 extern "C" {
@@ -1348,6 +1490,18 @@ int fedtrain_act_backward(int dtype, int act, int64_t rows, int64_t cols, const 
   if (dtype == FEDTRAIN_F32) return slope<FEDTRAIN_F32>(act, x, s);
   if (dtype == FEDTRAIN_BF16) return slope<FEDTRAIN_BF16>(act, x, s);
   return slope<FEDTRAIN_F16>(act, x, s);
+}
+
+int64_t fedtrain_act_backward_sums_workspace(const fedtrain_act_args* args) {
+  return valid(args) ? workspace(*args) : FEDTRAIN_EINVAL;
+}
+
+int fedtrain_act_backward_sums(const fedtrain_act_args* args, void* stream) {
+  if (!valid(args)) return FEDTRAIN_EINVAL;
+  if (!args->cols) return 0;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (args->dtype == FEDTRAIN_BF16) return slope_sums<FEDTRAIN_BF16>(*args, s);
+  return slope_sums<FEDTRAIN_F16>(*args, s);
 }
 
 }  // extern "C"

@@ -21,7 +21,7 @@
 extern "C" {
 #endif
 
-#define FEDTRAIN_ABI_VERSION 2
+#define FEDTRAIN_ABI_VERSION 3
 #define FEDTRAIN_EINVAL (-22)
 
 #define FEDTRAIN_F32 0
@@ -89,6 +89,29 @@ int fedtrain_product_plan(const fedtrain_product_args* args, int* rows, int* col
 int fedtrain_act_backward(int dtype, int act, int64_t rows, int64_t cols, const void* dy,
                           int64_t lddy, const void* z, int64_t ldz, void* dz, int64_t lddz,
                           void* stream);
+
+/* The same for 16-bit types, and each group's bias gradient from the terms before
+ * they are rounded: colsum[j] = sum_rows dy act'(z).  groups, offsets and rows of no
+ * group as in fedtrain_product; groups = 0 sums all rows.  (float32's dz is not
+ * rounded, and FEDTRAIN_GRAD_WEIGHT sums it.) */
+typedef struct fedtrain_act_args {
+  int32_t dtype, act, groups, offsets64;
+  int64_t rows, cols;
+  const void* dy;
+  int64_t lddy;
+  const void* z;
+  int64_t ldz;
+  void* dz;
+  int64_t lddz;
+  void* colsum; /* [cols] a group */
+  int64_t colsum_group;
+  const void* offsets;
+  void* workspace; /* fedtrain_act_backward_sums_workspace bytes, 16-byte aligned */
+  int64_t workspace_bytes;
+} fedtrain_act_args;
+
+int64_t fedtrain_act_backward_sums_workspace(const fedtrain_act_args* args);
+int fedtrain_act_backward_sums(const fedtrain_act_args* args, void* stream);
 
 /* One tensor of an AdamW step: n elements; g has p's type; m and v are f32
  * (state_bits 32), or e4m3 and e5m2 codes with one f32 scale for each 256

@@ -130,3 +130,46 @@ def test_float32_factors_next_to_the_smallest(tiny):
     S = x.double().abs() @ w.double().abs().T
     e = R.sum_error(64, S) + 2.0 ** -125 * w.double().abs().sum(1)[None] + 64 * R.TINY[torch.float32]
     R.close(y, (x.double() @ w.double().T, e.expand(40, 24)), str(tiny))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("act", ["relu", "gelu", "silu"])
+@pytest.mark.parametrize("case", [(777, 333, None), (1, 40, None), (2048, 65, None),
+                                  (2049, 8, None), (9000, 130, None), (0, 9, None),
+                                  (700, 136, [0, 300, 300, 301, 700]),
+                                  (9000, 70, [5, 2100, 2100, 8800]), (64, 12, [0] * 40 + [60])],
+                         ids=str)
+def test_bias_gradients_are_sums_of_unrounded_terms(case, act, dtype):
+    """db in 16 bits: the terms dy act'(z) are not rounded on their way.  x is one
+    value a row and w is 1, so z is x, which its type holds: float32's slope (16
+    units of 2^-24 of 1 + |z|, and relu's none) and sum are all that is between db
+    and the definition's, rounded once."""
+    from fedsim_amd.functional import grouped_linear, linear_act
+
+    N, M, edges = case
+    gen = torch.Generator().manual_seed(N + M)
+    x = torch.randn(N, 1, generator=gen).to(dtype)
+    dy = torch.randn(N, M, generator=gen).to(dtype)
+    G = len(edges) - 1 if edges else 1
+    w = torch.ones(G, M, 1, dtype=dtype, device=DEV)
+    B = torch.zeros(G, M, dtype=dtype, device=DEV, requires_grad=True)
+    X = x.to(DEV).requires_grad_(True)
+    if edges:
+        y = grouped_linear(X, w, torch.tensor(edges, device=DEV), B, activation=act)
+    else:
+        y = linear_act(X, w[0], B[0], activation=act)
+    db, dx = torch.autograd.grad(y, (B, X), dy.to(DEV))
+    z = x.double().expand(N, M)
+    dz = dy.double() * R.slope(z, act)
+    unit = 0.0 if act == "relu" else 16 * 2.0 ** -24
+    term = dy.double().abs() * unit * (1 + z.abs())
+    for g, (lo, hi) in enumerate(zip(edges, edges[1:]) if edges else [(0, N)]):
+        v, s = dz[lo:hi].sum(0), dz[lo:hi].abs().sum(0)
+        e = term[lo:hi].sum(0) + R.sum_error(hi - lo, s)
+        R.close(db[g], (v, e + R.HALF[dtype] * (v.abs() + e) + R.TINY[dtype]), f"db {g}")
+        if hi == lo:
+            assert not db[g].any()
+    again = torch.autograd.grad(
+        grouped_linear(X, w, torch.tensor(edges, device=DEV), B, activation=act) if edges
+        else linear_act(X, w[0], B[0], activation=act), B, dy.to(DEV))[0]
+    assert torch.equal(again, db)

@@ -34,6 +34,43 @@ def test_counts_on_the_device_are_checked():
         assert call(**kw) == E, kw
 
 
+def test_act_backward_sums_refusals():
+    from fedsim_amd import _native_train as nt
+
+    lib = nt.load()
+
+    def args(**kw):
+        d = dict(dtype=1, act=2, rows=10, cols=4, dy=64, lddy=4, z=64, ldz=4, dz=64, lddz=4,
+                 colsum=64)
+        d.update(kw)
+        return ctypes.byref(nt.ActArgs(**d))
+
+    size = lib.fedtrain_act_backward_sums_workspace
+    assert size(args()) == size(args(rows=2048)) == size(args(rows=0)) == 0
+    assert size(args(rows=2049)) == 2 * 4 * 4
+    grouped = dict(groups=3, offsets=64, colsum_group=4)
+    assert size(args(**grouped)) == 5 * 4 * 4
+    assert size(args(rows=5000, **grouped)) == 7 * 4 * 4
+    call = lib.fedtrain_act_backward_sums
+    assert call(args(cols=0), None) == call(args(cols=0, dy=None, z=None, dz=None, colsum=None),
+                                            None) == 0
+    assert call(None, None) == size(None) == E
+    for bad in (dict(dtype=0), dict(dtype=3), dict(act=4), dict(act=-1), dict(groups=-1),
+                dict(groups=2147483647, offsets=64), dict(rows=-1), dict(cols=-1),
+                dict(rows=1 << 31), dict(cols=1 << 31), dict(dy=None), dict(z=None), dict(dz=None),
+                dict(colsum=None), dict(dy=65), dict(z=65), dict(dz=65), dict(colsum=65),
+                dict(lddy=-1), dict(ldz=-1), dict(lddz=3), dict(groups=2),
+                dict(groups=2, offsets=66, colsum_group=4),
+                dict(groups=2, offsets=68, offsets64=1, colsum_group=4),
+                dict(groups=2, offsets=64, colsum_group=3)):
+        assert call(args(**bad), None) == E and size(args(**bad)) == E, bad
+    for bad in (dict(rows=2049), dict(**grouped), dict(rows=2049, workspace=68, workspace_bytes=32),
+                dict(rows=2049, workspace=64, workspace_bytes=31),
+                dict(rows=1 << 30, cols=1 << 20, lddz=1 << 20, workspace=64,
+                     workspace_bytes=1 << 62)):
+        assert call(args(**bad), None) == E and size(args(**bad)) > 0, bad
+
+
 def _calls():
     """(name, function of two tensors, its arguments' shapes)."""
     from fedsim_amd import train_ops
