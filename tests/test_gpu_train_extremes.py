@@ -132,6 +132,29 @@ def test_float32_factors_next_to_the_smallest(tiny):
     R.close(y, (x.double() @ w.double().T, e.expand(40, 24)), str(tiny))
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "silu"])
+def test_the_call_that_keeps_nothing_gives_the_same_bits(act, dtype):
+    """With autograd off no z is stored; NaN are where they were."""
+    from fedsim_amd.functional import linear_act
+
+    gen = torch.Generator().manual_seed(33)
+    for N, K, M in ((3, 40, 70), (70, 96, 136), (600, 520, 520), (300, 33, 129)):
+        x = torch.randn(N, K, generator=gen).to(dtype)
+        x[N // 2, 1], x[0, 3] = float("nan"), float("inf")
+        w = torch.randn(M, K, generator=gen).to(dtype).to(DEV)
+        b = torch.randn(M, generator=gen).to(dtype).to(DEV)
+        r = torch.randn(N, M, generator=gen).to(dtype).to(DEV)
+        X = x.to(DEV).requires_grad_(True)
+        kept = linear_act(X, w, b, r, activation=act).detach()
+        with torch.no_grad():
+            bare = linear_act(X, w, b, r, activation=act)
+        assert kept[N // 2].isnan().all()
+        i = torch.int32 if dtype == torch.float32 else torch.int16
+        assert torch.equal(kept.isnan(), bare.isnan())
+        assert torch.equal(kept.nan_to_num(7.0).view(i), bare.nan_to_num(7.0).view(i))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
 @pytest.mark.parametrize("act", ["relu", "gelu", "silu"])
 @pytest.mark.parametrize("case", [(777, 333, None), (1, 40, None), (2048, 65, None),
