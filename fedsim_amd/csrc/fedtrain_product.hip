@@ -1037,36 +1037,71 @@ __global__ __launch_bounds__(256) void k_act_backward(int64_t rows, int64_t cols
 // The same where a bias wants its gradient too, in 16-bit types: its terms are added
 // up before they are rounded (rounded ones put db off 1.5 times as far as its own
 // rounding does, by several of its units where the terms cancel).  A workgroup takes
-// 64 columns of up to kSumRows rows of a group, 8 values a thread and 128 rows at a
+// 64 columns of up to 2^LOG rows of a group, 8 values a thread and 32 rows at a
 // time; sums go through the wave, LDS and, where there is more than one such part,
-// the workspace, in the same order in every run.
-constexpr int kSumRows = 2048, kSumCols = 64;
+// the workspace, in the same order in every run.  Memory and the slope's instructions
+// bound it: 8192 x 16384 bf16 gelu in 149 us and 10 to join, where k_act_backward takes
+// 130 and the grad weight's sums by the matrix unit 40; 777 x 333 f16 in 8.5 and 4.
+constexpr int kSumCols = 64;
+
+// rows_of() in parts of 2^log rows, the ranges looked at 64 at a time: the last one
+// whose slots begin at or before this.
+__device__ inline Rows part_of(const Args& a, int64_t slot, int log) {
+  int64_t first = 0, end = a.m;
+  int at = 0;
+  if (a.groups) {
+    const int n = a.groups + 2, lane = threadIdx.x & 63;
+    for (int i0 = 0; i0 < n; i0 += 64) {
+      const int i = i0 + lane;
+      const uint64_t m =
+          __builtin_amdgcn_ballot_w64(i < n && (bound(a, a.m, i) >> log) + i <= slot);
+      if (m) at = i0 + 63 - __builtin_clzll(m);
+    }
+    first = bound(a, a.m, at);
+    end = bound(a, a.m, at + 1);
+  }
+  const int64_t lo = first + ((slot - (first >> log) - at) << log), hi = lo + (1ll << log);
+  return {lo, hi < end ? hi : end, at};
+}
 
 template <int D, int ACT, bool ONCE>
-__global__ __launch_bounds__(1024) void k_act_backward_sums(Args a, int64_t strips, bool joined) {
+__global__ __launch_bounds__(256) void k_act_backward_sums(Args a, unsigned strips, int log,
+                                                           bool joined) {
   using T = typename Elem<D>::type;
-  __shared__ float part[16][kSumCols];
-  const int64_t slot = blockIdx.x / strips, col0 = blockIdx.x % strips * kSumCols;
-  const Rows taken = rows_of(a, slot, kSumRows);
+  __shared__ float part[4][kSumCols];
+  const int64_t slot = blockIdx.x / strips;
+  const int64_t col0 = static_cast<int64_t>(blockIdx.x % strips) * kSumCols;
+  const Rows taken = part_of(a, slot, log);
   if (joined && taken.lo >= taken.hi) return;
   const int lane = threadIdx.x & 63, c = (threadIdx.x & 7) * 8;
   const int64_t col = col0 + c;
   const int n = static_cast<int>(a.n - col < 8 ? a.n - col : 8);
   float sum[8] = {};
-  if (n > 0) {
-#pragma unroll 2
-    for (int64_t r = taken.lo + (threadIdx.x >> 3); r < taken.hi; r += 128) {
-      float g[8], x[8];
-      read8<D>(a.a, r * a.lda + col, n, g);
-      read8<D>(a.b, r * a.ldb + col, n, x);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        g[e] *= act_slope<D, ACT>(x[e]);
-        sum[e] += g[e];
+  // two rows' loads before their sums
+  auto pass = [&](int n) {
+    for (int64_t r = taken.lo + (threadIdx.x >> 3); r < taken.hi; r += 64) {
+      const bool both = r + 32 < taken.hi;
+      float g[2][8], x[2][8];
+      read8<D>(a.a, r * a.lda + col, n, g[0]);
+      read8<D>(a.b, r * a.ldb + col, n, x[0]);
+      if (both) {
+        read8<D>(a.a, (r + 32) * a.lda + col, n, g[1]);
+        read8<D>(a.b, (r + 32) * a.ldb + col, n, x[1]);
       }
-      write8<D, ONCE>(static_cast<T*>(a.c) + r * a.ldc + col, n, g);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (j && !both) break;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          g[j][e] *= act_slope<D, ACT>(x[j][e]);
+          sum[e] += g[j][e];
+        }
+        write8<D, ONCE>(static_cast<T*>(a.c) + (r + j * 32) * a.ldc + col, n, g[j]);
+      }
     }
-  }
+  };
+  if (n >= 8) pass(8);
+  else if (n > 0) pass(n);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
 #pragma unroll
@@ -1077,27 +1112,27 @@ __global__ __launch_bounds__(1024) void k_act_backward_sums(Args a, int64_t stri
   if (threadIdx.x >= kSumCols || col0 + threadIdx.x >= a.n) return;
   float all = 0;
 #pragma unroll
-  for (int w = 0; w < 16; ++w) all += part[w][threadIdx.x];
+  for (int w = 0; w < 4; ++w) all += part[w][threadIdx.x];
   if (joined) static_cast<float*>(a.workspace)[slot * a.n + col0 + threadIdx.x] = all;
   else static_cast<T*>(a.colsum)[col0 + threadIdx.x] = Elem<D>::down(all);
 }
 
 // A group's parts, a thread for each of its columns.
-template <int D> __global__ __launch_bounds__(256) void k_sums_join(Args a) {
+template <int D> __global__ __launch_bounds__(256) void k_sums_join(Args a, int log) {
   using T = typename Elem<D>::type;
   const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (id >= (a.groups ? a.groups : 1) * a.n) return;
   const int64_t group = id / a.n, col = id % a.n;
   int64_t lo = 0, hi = a.m, slot = 0;
-  if (a.groups) {  // as rows_of() deals them out
+  if (a.groups) {  // as part_of() deals them out
     const int i = static_cast<int>(group) + 1;
     lo = bound(a, a.m, i);
     hi = bound(a, a.m, i + 1);
-    slot = lo / kSumRows + i;
+    slot = (lo >> log) + i;
   }
   float all = 0;
-#pragma unroll 4
-  for (; lo < hi; lo += kSumRows, ++slot)
+#pragma unroll 8
+  for (; lo < hi; lo += 1ll << log, ++slot)
     all += static_cast<const float*>(a.workspace)[slot * a.n + col];
   static_cast<T*>(a.colsum)[group * a.colsum_group + col] = Elem<D>::down(all);
 }
@@ -1379,13 +1414,24 @@ bool valid(const fedtrain_act_args* x) {
   return !x->cols || (x->colsum && (!x->rows || (x->dy && x->z && x->dz)));
 }
 
+// Rows of a part, as a power of two: 32, so that small cases fill the card; more where
+// there would be over 256 parts, which k_sums_join adds up one by one, or over 128
+// workgroups a compute unit (8192 x 16384 bf16 with 128, 64 and 32 rows: 166, 148 and
+// 182 us, and 6, 10 and 17 to join).
+int sum_log(const fedtrain_act_args& x) {
+  const int64_t strips = (x.cols + kSumCols - 1) / kSumCols;
+  int log = 5;
+  while (x.rows >> log > 256 || (x.rows >> log) * strips > 128 * 256) ++log;
+  return log;
+}
 // Parts of rows, and whether their sums have to be joined: not where one workgroup
 // sees all rows of its columns.
 int64_t sum_slots(const fedtrain_act_args& x) {
-  if (x.groups) return x.rows / kSumRows + x.groups + 2;
-  return std::max<int64_t>(1, (x.rows + kSumRows - 1) / kSumRows);
+  const int log = sum_log(x);
+  if (x.groups) return (x.rows >> log) + x.groups + 2;
+  return std::max<int64_t>(1, (x.rows + (1ll << log) - 1) >> log);
 }
-bool sums_joined(const fedtrain_act_args& x) { return x.groups || x.rows > kSumRows; }
+bool sums_joined(const fedtrain_act_args& x) { return x.groups || sum_slots(x) > 1; }
 
 int64_t workspace(const fedtrain_act_args& x) {
   return sums_joined(x) ? sum_slots(x) * x.cols * 4 : 0;
@@ -1395,8 +1441,9 @@ template <int D, int ACT> int slope_sums(const fedtrain_act_args& x, hipStream_t
   const int64_t strips = (x.cols + kSumCols - 1) / kSumCols, slots = sum_slots(x);
   const int64_t sums = (x.groups ? x.groups : 1) * x.cols;
   const bool joined = sums_joined(x);
+  const int log = sum_log(x);
   // a launch's threads are counted in 32 bits
-  if (slots > UINT32_MAX / 1024 / strips || sums > kMostGroups * 256) return FEDTRAIN_EINVAL;
+  if (slots > kMostGroups / strips || sums > kMostGroups * 256) return FEDTRAIN_EINVAL;
   if (joined && (!x.workspace || !aligned(x.workspace, 16) || x.workspace_bytes < workspace(x)))
     return FEDTRAIN_EINVAL;
   Args a = {};
@@ -1416,12 +1463,12 @@ template <int D, int ACT> int slope_sums(const fedtrain_act_args& x, hipStream_t
   a.workspace = x.workspace;
   auto* kernel = written_once<D>(x.rows * x.cols) ? &k_act_backward_sums<D, ACT, true>
                                                   : &k_act_backward_sums<D, ACT, false>;
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(slots * strips)), dim3(1024), 0, s, a,
-                     strips, joined);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(slots * strips)), dim3(256), 0, s, a,
+                     static_cast<unsigned>(strips), log, joined);
   if (joined) {
     if (const int rc = launched()) return rc;
     hipLaunchKernelGGL((k_sums_join<D>), dim3(static_cast<unsigned>((sums + 255) / 256)),
-                       dim3(256), 0, s, a);
+                       dim3(256), 0, s, a, log);
   }
   return launched();
 }

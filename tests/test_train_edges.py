@@ -46,11 +46,13 @@ def test_act_backward_sums_refusals():
         return ctypes.byref(nt.ActArgs(**d))
 
     size = lib.fedtrain_act_backward_sums_workspace
-    assert size(args()) == size(args(rows=2048)) == size(args(rows=0)) == 0
-    assert size(args(rows=2049)) == 2 * 4 * 4
+    assert size(args()) == size(args(rows=32)) == size(args(rows=0)) == 0
+    assert size(args(rows=33)) == 2 * 4 * 4
     grouped = dict(groups=3, offsets=64, colsum_group=4)
     assert size(args(**grouped)) == 5 * 4 * 4
-    assert size(args(rows=5000, **grouped)) == 7 * 4 * 4
+    assert size(args(rows=5000, **grouped)) == (5000 // 32 + 5) * 4 * 4
+    assert size(args(rows=1 << 20)) == 256 * 4 * 4  # no more parts than that
+    assert size(args(rows=8192, cols=16384, lddz=16384)) == 128 * 16384 * 4
     call = lib.fedtrain_act_backward_sums
     assert call(args(cols=0), None) == call(args(cols=0, dy=None, z=None, dz=None, colsum=None),
                                             None) == 0
@@ -64,11 +66,12 @@ def test_act_backward_sums_refusals():
                 dict(groups=2, offsets=68, offsets64=1, colsum_group=4),
                 dict(groups=2, offsets=64, colsum_group=3)):
         assert call(args(**bad), None) == E and size(args(**bad)) == E, bad
-    for bad in (dict(rows=2049), dict(**grouped), dict(rows=2049, workspace=68, workspace_bytes=32),
-                dict(rows=2049, workspace=64, workspace_bytes=31),
-                dict(rows=1 << 30, cols=1 << 20, lddz=1 << 20, workspace=64,
-                     workspace_bytes=1 << 62)):
+    for bad in (dict(rows=33), dict(**grouped), dict(rows=33, workspace=68, workspace_bytes=32),
+                dict(rows=33, workspace=64, workspace_bytes=31)):
         assert call(args(**bad), None) == E and size(args(**bad)) > 0, bad
+    # more workgroups than a launch holds
+    wide = args(rows=1 << 20, cols=(1 << 31) - 1, lddz=1 << 31)
+    assert size(wide) == 0 and call(wide, None) == E
 
 
 def _calls():
