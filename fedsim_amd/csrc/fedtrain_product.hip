@@ -19,14 +19,16 @@
 // reaches 4.64 TB/s, the library's product of 8192^3 bf16 1.31 and f32 0.15
 // PFLOP/s):
 //   large 16-bit products   the matrix unit at the clock that power leaves:
-//                           8192 x 4096 x 16384 bf16 in 830 to 990 us, 1.11 to
+//                           8192 x 4096 x 16384 bf16 in 830 to 960 us, 1.14 to
 //                           1.32 PFLOP/s, in tiles of 256 x 256
-//   large f32 products      the same through six bf16 products each: 2048 x 512 x
-//                           3136 in 53 to 60 us with parts of k, 200 TFLOP/s at
-//                           larger sizes
-//   1000 clients' weights   memory: 3.5 GB of weights read once, 0.94 ms
-//   64 experts              tiles that ragged groups fill by two thirds: 520 to 710
-//                           us, of 400 by memory and 290 by the matrix unit
+//   large f32 products      six bf16 products each: 194 TFLOP/s at 8192^3; 2048 x 512
+//                           x 3136 in 54 to 59 us, 111 to 122 TFLOP/s, and 7 to 8 for
+//                           parts of k: with few workgroups on a compute unit a
+//                           step's loads, split and two barriers are its time
+//   1000 clients' weights   memory: 3.5 GB of weights read once, 0.82 to 0.96 ms
+//   64 experts              tiles that ragged groups fill by two thirds: forward 610
+//                           us, grad input 510, of 400 by memory and 290 by the matrix
+//                           unit; grad weight 720 to 850, four steps of k a tile
 //   a client's small batch  launches and the trip to memory: 5 to 9 us each
 #include "fedtrain_common.h"
 
@@ -597,13 +599,13 @@ template <int D, int FORM> struct Out {
 };
 
 // A workgroup's tile of C.  16-bit operands whose chunks are whole and aligned go to
-// LDS directly (DIRECT): no registers and no instructions of the waves, which keeps
-// 256 sums a lane in registers of the largest tile and the matrix unit busy for 75 %
-// of a steady run's cycles (57 % with a stage's reads ahead of its products).  A tile of 256 x 256 by
-// four waves reads 64 bytes of LDS for each product, half of what eight waves
+// LDS directly (DIRECT): no registers and no instructions of the waves, which leaves
+// room for 256 sums a lane of the largest tile; the matrix unit is busy for 54 to 62 %
+// of its products' cycles, counted one at a time on a rested card.  A tile of 256 x
+// 256 by four waves reads 64 bytes of LDS for each product, half of what eight waves
 // would (30 % slower) and a quarter of what 128 x 128 by four does.  Operands at
 // any other alignment, and f32 on its way into three parts, come through
-// registers: 1003 x 517 f16 at odd strides 30 to 41 us a product where memory
+// registers: 1003 x 517 f16 at odd strides 33 to 41 us a product where memory
 // needs about 9.
 template <int D, int FORM, class S> __global__ __launch_bounds__(S::THREADS, S::WAVES)
 void k_product(Args a, Plan plan) {
@@ -1014,8 +1016,7 @@ __global__ __launch_bounds__(256) void k_few_rows(Args a) {
 }
 
 // dz = dy act'(z): one pass, eight values of a row a thread, at any alignment.
-// Memory bounds it: 16384 x 5632 bf16 in 91 us and 8192 x 16384 in 130 (6.1 TB/s),
-// less where dy and z are still in the caches.
+// Memory bounds it: 16384 x 5632 bf16 in 90 us and 8192 x 16384 in 131 (6.1 TB/s).
 template <int D, int ACT, bool ONCE>
 __global__ __launch_bounds__(256) void k_act_backward(int64_t rows, int64_t cols, const void* dy,
                                                       int64_t lddy, const void* z, int64_t ldz,
@@ -1041,7 +1042,7 @@ __global__ __launch_bounds__(256) void k_act_backward(int64_t rows, int64_t cols
 // time; sums go through the wave, LDS and, where there is more than one such part,
 // the workspace, in the same order in every run.  Memory and the slope's instructions
 // bound it: 8192 x 16384 bf16 gelu in 149 us and 10 to join, where k_act_backward takes
-// 130 and the grad weight's sums by the matrix unit 40; 777 x 333 f16 in 8.5 and 4.
+// 130; 777 x 333 f16 in 8.5 and 4.
 constexpr int kSumCols = 64;
 
 // rows_of() in parts of 2^log rows, the ranges looked at 64 at a time: the last one
@@ -1250,9 +1251,10 @@ Choice choose(const Args& a) {
 }
 
 // Up to 4 rows of one weight matrix, while reading the weights costs more than the
-// vector unit's products.  4096 x 4096: one bf16 row 8.8 us, on the matrix unit
-// 12; two 12.1 and 11.9, four 15.4 and 11.9; four f32 rows 20 and 25.  784 x 200:
-// 4 to 5 us, in place of 8 (bf16) and 11 (f32) by parts of k and their sum.
+// vector unit's products.  4096 x 4096, the weights in the caches: one bf16 row 5.1 us
+// (9 from memory), on the matrix unit 11.5; two 12.1 and 11.9, four 15.4 and 11.9; one,
+// two and four f32 rows 12.3, 13.3 and 16.3, on the matrix unit 21.  784 x 200: 4 to 5
+// us, in place of 7 (bf16) and 10 (f32) by parts of k and their sum.
 bool few_rows(const Args& a) {
   return a.form == FEDTRAIN_FORWARD && !a.groups && a.m <= 4 && a.n < 1 << 28 &&
          (a.dtype == FEDTRAIN_F32 || a.m == 1 ||
@@ -1267,8 +1269,8 @@ int64_t workspace(const Args& a) {
 }
 
 // Results this large are not in the caches (256 MB) when they are read next, and
-// push out what is: storing past them took 64 experts' grad weight from 800 to
-// 700 us, 1000 clients' from 1370 to 1200, dz of 8192 x 16384 from 118 to 91.
+// push out what is: storing past them takes 64 experts' grad weight from 820 to 720
+// us, dz of 8192 x 16384 and 16384 x 5632 from 133 to 131 and from 93 to 90.
 template <int D> bool written_once(int64_t values) {
   return values * static_cast<int64_t>(sizeof(typename Elem<D>::type)) >= 128 << 20;
 }

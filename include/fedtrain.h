@@ -4,7 +4,7 @@
  *                          the epilogue, of one weight matrix or grouped by
  *                          client with ragged row counts, and the products of
  *                          their gradients
- *   fedtrain_act_backward  the activation's gradient
+ *   fedtrain_act_backward  the activation's gradient; with _sums, a bias's too
  *   fedtrain_adamw         an AdamW step over many tensors, states in 32 or 8 bits
  *
  * Every entry checks its arguments on the host, launches on `stream` (a
