@@ -65,7 +65,8 @@ __device__ inline float phi_of(float z, float e) {
   return z < 0 ? half : 1.0f - half;
 }
 
-// The same for f32, by the library's erfc.
+// The same for f32, by the library's erfc: 8192 x 8192 outputs of 256 inputs 276 us and
+// their gradient's pass 146, where erff, which cancels, made 253 and 137.
 __device__ inline float phi(float z) { return 0.5f * erfcf(z * -0.70710678118654752f); }
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -1038,7 +1039,7 @@ __global__ __launch_bounds__(256) void k_act_backward(int64_t rows, int64_t cols
 // The same where a bias wants its gradient too, in 16-bit types: its terms are added
 // up before they are rounded (rounded ones put db off 1.5 times as far as its own
 // rounding does, by several of its units where the terms cancel).  A workgroup takes
-// 64 columns of up to 2^LOG rows of a group, 8 values a thread and 32 rows at a
+// 64 columns of up to 2^log rows of a group, 8 values a thread and 32 rows at a
 // time; sums go through the wave, LDS and, where there is more than one such part,
 // the workspace, in the same order in every run.  Memory and the slope's instructions
 // bound it: 8192 x 16384 bf16 gelu in 149 us and 10 to join, where k_act_backward takes
